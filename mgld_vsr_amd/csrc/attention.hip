@@ -453,7 +453,7 @@ void flash_attn_kernel(const MgldAttn p, const int xcd_order) {
 //     probabilities of the tile sum to more than 2^11 (or to inf / NaN) raises the rare branch, which works on the kept raw scores:
 //     exact row max (with the lane^32 exchange), m += delta for rows more than PS_THR above it, o, l, the new probabilities and the
 //     already accumulated scores of tile t+1 all take the same delta.  Without the branch every p <= 2^11 (fp16-safe); the two half-row
-//     partial sums of l meet only in the epilogue.  VALU per wave-tile: 32 v_exp + 16 v_pk_add + 16 v_cvt_pk + ~16 others: 96
+//     partial sums of l meet only in the epilogue.  VALU per wave-tile: 32 v_exp + 32 v_add + 16 v_cvt_pk + ~16 others: 112
 //     instructions, 512 port cycles (was 167 / ~800).
 //  3. RING: K / V tiles go through a three-slot LDS ring of "shifted tiles" {K(j+1), V(j)} (what iteration j reads), issued TWO
 //     iterations ahead with a counted vmcnt(4) — the newest tile's four pieces stay in flight across the barrier.
@@ -652,7 +652,7 @@ void flash_attn_sp_kernel(const MgldAttn p, const int xcd_order) {
         for (int j = 0; j < 2; ++j) {
           const f32x2 ep = {e[g * 4 + 2 * j], e[g * 4 + 2 * j + 1]};
           if (g == 0) rsq[j] = ep;
-          else asm("v_pk_add_f32 %0, %1, %0" : "+v"(rsq[j]) : "v"(ep));
+          else rsq[j] += ep;
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -911,10 +911,10 @@ void flash_attn_sp2_kernel(const MgldAttn p, const int xcd_order) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[g * 4 + j] = __builtin_amdgcn_exp2f(sa[g >> 2][(g & 3) * 4 + j]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {    // (row sums as two packed adds per gap; four plain v_add_f32 measured the same)
+        for (int j = 0; j < 2; ++j) {    // (row sums: four v_add_f32 per gap; two packed adds measured the same)
           const f32x2 ep = {e[g * 4 + 2 * j], e[g * 4 + 2 * j + 1]};
           if (g == 0) rsq[j] = ep;
-          else asm("v_pk_add_f32 %0, %1, %0" : "+v"(rsq[j]) : "v"(ep));
+          else rsq[j] += ep;
         }
       }
       __builtin_amdgcn_sched_barrier(0);

@@ -127,7 +127,7 @@ __device__ __forceinline__ e2 silu2(e2 x) {
 }
 // exact-GELU of a pair: erf(z) = sign(z) (1 - 2^(t q(t))), t = min(|z|, 4), q a degree-5 polynomial fitted to log2(erfc(t)) / t on [0, 4]
 // (weighted minimax, tools/fit_erf.py; |erf error| <= 2.9e-7 in fp32 Horner: fp32 round-off level, three orders below the fp16 rounding of
-// the stored product).  One transcendental (v_exp_f32) per element; the polynomial runs as v_pk_fma_f32 on the pair.
+// the stored product).  One transcendental (v_exp_f32) per element; the polynomial runs on the pair.
 __device__ __forceinline__ e2 gelu2(e2 x) {
   const e2 z = x * pk(0.70710678118654752440f, 0.70710678118654752440f);
   const e2 t = pk(fminf(fabsf(z[0]), 4.f), fminf(fabsf(z[1]), 4.f));
@@ -362,7 +362,7 @@ __device__ __forceinline__ void tile_epilogue(const MgldIGemm& p, float* __restr
                   acc[c * NIC + nic][mi][rg * 4 + 3]};
     // ---- phase 2: patch rows -> epilogue math -> global, 8 columns (16 B of fp16 / 32 B of fp32) per lane ----
     // The variant (plain fp16 epilogue with a compile-time activation / GEGLU / raw split-K slab / everything else) is picked by
-    // ONE block-uniform switch per 32-row slice; inside, the arithmetic is straight-line packed fp32 (v_pk_add/mul/fma_f32).
+    // ONE block-uniform switch per 32-row slice; inside, the arithmetic is straight-line fp32 on pairs.
     // Short-K launches (K = 320..1280: 5-20 k-steps) spend more issue slots here than in the k loop, so a per-element
     // runtime `act` switch (4 scalar branches per element) was the dominant cost of the transformer blocks' projections.
     switch (kind) {

@@ -265,7 +265,7 @@ __device__ __forceinline__ void pp_epilogue_stats(const PPEpi& e, f32x4 (&acc)[N
   };
 #pragma unroll
   for (int pr = 0; pr < NI / 2; ++pr) {
-    e2 ss[4], qq[4];                                             // packed fp32 pairs: v_pk_add_f32 / v_pk_fma_f32
+    e2 ss[4], qq[4];                                             // fp32 pairs
 #pragma unroll
     for (int r = 0; r < 4; ++r) { ss[r] = pk(0.f, 0.f); qq[r] = pk(0.f, 0.f); }
     const int nl = (2 * pr + (q & 1)) * 16 + (q >> 1) * 8;       // this lane's 8 channels of the wave tile after the swap
