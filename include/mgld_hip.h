@@ -458,6 +458,79 @@ int mgld_hp_gn_split(const float* x, int ldx, const double* gsums, float eps, co
 /* in-place softmax over the `cols` entries of every fp32 row (the mid attention's key axis, model.py:226-229) */
 int mgld_hp_softmax_rows(float* S, int64_t rows, int cols, int ld, void* stream);
 
+/* ---- operators of transformer blocks beside the ones the pipeline runs (fp16 or bf16, fp32 statistics) --------------------------------
+ * A "heads" view is [rows, heads, head_dim] with unit stride along head_dim and any row / head strides (elements): the column blocks of a
+ * fused projection, [batch, position, head, d] or [batch, head, position, d] tensors.  16-byte aligned pointers and strides that are
+ * multiples of 8 elements unless said otherwise.  bf16 = 1: every fp16 tensor of the call is bfloat16. */
+/* Root-mean-square norm of each query and key head (n = x (mean_d x^2 + eps)^-1/2 gamma) and the position rotation of its first rot_dim
+ * elements, in one pass: pair j of row p turns by pos[p] * freqs[j] (fp64).  Pairs: (j, j + rot_dim / 2), or interleaved = 1: (2 j, 2 j + 1).
+ * x == y (in place) allowed.  head_dim and rot_dim multiples of 8, head_dim <= 256; 8-byte alignment suffices (16 is faster).
+ * A side with heads = 0 is skipped. */
+typedef struct MgldHeads {
+  const void* x;       /* [rows, heads, head_dim]: the projection's output (the forward input, also for the gradient)      */
+  void* y;             /* forward: the result; gradient: dx                                                               */
+  const void* dy;      /* gradient: of the result                                                                         */
+  const float* gamma;  /* [head_dim] or NULL (ones)                                                                       */
+  float* dgamma;       /* gradient: [head_dim], overwritten, or NULL                                                      */
+  int64_t x_sr, x_sh, y_sr, y_sh, dy_sr, dy_sh;
+  int64_t heads;
+} MgldHeads;
+typedef struct MgldQkRope {
+  MgldHeads q, k;
+  const void* pos;       /* [rows] int64 (pos64 = 1) or int32; NULL with rot_dim = 0 */
+  const double* freqs;   /* [rot_dim / 2] radians per position */
+  float* work;           /* gradient with a dgamma: mgld_qk_norm_rope_grad_work bytes, 16-byte aligned */
+  int64_t work_bytes, rows;
+  int32_t pos64, head_dim, rot_dim, interleaved, bf16;
+  float eps;
+} MgldQkRope;
+int mgld_qk_norm_rope(const MgldQkRope* p, void* stream);
+int64_t mgld_qk_norm_rope_grad_work(const MgldQkRope* p);
+/* z = R^T dy; dgamma = sum over rows and heads of z x r (fp32 per block, fp64 over the blocks, fixed order);
+ * dx = r (gamma z - x r mean_d(gamma z x r)).  dx may be dy or x. */
+int mgld_qk_norm_rope_grad(const MgldQkRope* p, void* stream);
+
+/* Attention with capped scores, distance biases and masks.  For query i of batch row b, standing at position p_i = i + q_pos0 (or, with
+ * q_from_end, i + len_b - Nq), and key j < len_b (len_b = kv_len[b] clamped to [0, Nkv], or Nkv):
+ *   t = scale q.k;  u = softcap tanh(t / softcap) if softcap > 0, else t;  s = u - slopes[h] |j - p_i| + rel[h][clamp(j - p_i, -reach, reach) + reach]
+ *   visible: j < len_b, and (causal: j <= p_i or j < prefix[b]), and (documents: doc_q[i] == doc_k[j] >= 0)
+ *   o = sum_visible softmax(s) v,  lse = log sum_visible exp(s);   a query that sees nothing: o = 0, lse = -inf, and no gradient.
+ * A value or key that a query does not see never reaches that query's result, whatever it holds (infinities, NaN).
+ * heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads). */
+typedef struct MgldMaskAttn {
+  const void* Q; const void* K; const void* V; void* O;
+  float* lse;                       /* [batch, heads, Nq] contiguous, or NULL (forward only)                                */
+  int64_t q_sb, q_si, q_sh, k_sb, k_si, k_sh, v_sb, v_si, v_sh, o_sb, o_si, o_sh;
+  const float* slopes;              /* [heads] or NULL                                                                      */
+  const float* rel;                 /* [heads, 2 * reach + 1] or NULL; reach <= 1024; not together with slopes               */
+  const int32_t* doc_q; const int32_t* doc_k;   /* [batch, Nq], [batch, Nkv], unit stride, both or neither                  */
+  const int32_t* prefix;            /* [batch] or NULL; needs causal                                                        */
+  const int32_t* kv_len;            /* [batch] or NULL                                                                      */
+  int64_t doc_q_sb, doc_k_sb;         /* batch strides of doc_q / doc_k                                                       */
+  /* gradient */
+  const void* dO; void* dQ; void* dK; void* dV;
+  float* dRel;                      /* [heads, 2 * reach + 1], overwritten, or NULL                                         */
+  int64_t do_sb, do_si, do_sh, dq_sb, dq_si, dq_sh, dk_sb, dk_si, dk_sh, dv_sb, dv_si, dv_sh;
+  void* work;                       /* mgld_masked_attention_work / _grad_work bytes, 16-byte aligned; NULL if that is 0    */
+  int64_t work_bytes;
+  int32_t batch, heads, kv_heads, Nq, Nkv, head_dim;    /* head_dim: a multiple of 8 up to 128 */
+  int32_t reach, q_pos0, q_from_end, causal, bf16;
+  float scale, softcap;             /* scale > 0; softcap 0: none */
+} MgldMaskAttn;
+int64_t mgld_masked_attention_work(const MgldMaskAttn* p);
+int mgld_masked_attention(const MgldMaskAttn* p, void* stream);
+/* From the forward's o and lse: dV = P^T dO, dS = P (dO V^T - rowsum(dO o)), dRel = dS summed over rows, batch and equal distances,
+ * dQ = scale dT K, dK = scale dT^T Q with dT = dS (1 - (u / softcap)^2); K / V gradients summed over the query heads that share them.
+ * Every sum has a fixed order.  Rows of dK / dV that no query sees are written as zeros. */
+int64_t mgld_masked_attention_grad_work(const MgldMaskAttn* p);
+int mgld_masked_attention_grad(const MgldMaskAttn* p, void* stream);
+
+/* Learned relative bias by buckets: rel[h][i] = table[index[i]][h] for the n = 2 * reach + 1 distances (the layout MgldMaskAttn.rel reads),
+ * and its gradient dtable[b][h] = sum over the distances i with index[i] == b of drel[h][i], in a fixed order.  index: int32 [n], entries
+ * outside [0, buckets) give 0 / are skipped.  table: fp32 [buckets, heads]. */
+int mgld_rel_bias(const float* table, const int32_t* index, float* rel, int buckets, int heads, int n, void* stream);
+int mgld_rel_bias_grad(const float* drel, const int32_t* index, float* dtable, int buckets, int heads, int n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,7 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmgld_hip.so")
 STAMP = os.path.join(HERE, "csrc", ".build_stamp")
-SOURCES = ["runtime.hip", "igemm.hip", "conv3q.hip", "ppgemm.hip", "conv3r.hip", "pptconv.hip", "norm.hip", "attention.hip", "elementwise.hip", "raft.hip", "hpenc.hip"]
+SOURCES = ["runtime.hip", "igemm.hip", "conv3q.hip", "ppgemm.hip", "conv3r.hip", "pptconv.hip", "norm.hip", "attention.hip", "elementwise.hip", "raft.hip", "hpenc.hip",
+           "qkrope.hip", "maskattn.hip", "maskattn_grad.hip", "relbias.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result"]
 # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms give wrong results now and then on this hardware.  norm.hip keeps it:
 # without it the compiler contracts the normalisations' products differently, and the recorded results of the samplers move
@@ -42,7 +43,7 @@ def _file_digest(paths):
 
 
 def _common():
-    return [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "igemm_common.h"), os.path.join(CSRC, "pp_common.h"), os.path.join(HERE, "..", "include", "mgld_hip.h")]
+    return [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "igemm_common.h"), os.path.join(CSRC, "pp_common.h"), os.path.join(CSRC, "maskattn.h"), os.path.join(HERE, "..", "include", "mgld_hip.h")]
 
 
 def _digest():

@@ -1,0 +1,326 @@
+// maskattn.h — what the masked-attention kernels (maskattn.hip: forward, maskattn_grad.hip: gradient) share: operand types, the LDS image of a
+// tile, scores, visibility and the list of tiles that a group of query rows has to visit.
+#pragma once
+#include "common.h"
+
+namespace {
+
+typedef __bf16 bf16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) char* ma_lds;
+
+template <typename T> struct MaVec;
+template <> struct MaVec<f16> { typedef f16x8 v8; };
+template <> struct MaVec<bf16> { typedef bf16x8 v8; };
+__device__ __forceinline__ f32x16 ma_mfma(const f16x8 a, const f16x8 b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 ma_mfma(const bf16x8 a, const bf16x8 b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 ma_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+// eight fp32 values -> eight T, round to nearest even: the probabilities (and dS) become operands of the second product; their relative
+// rounding error (2^-9 bf16, 2^-12 fp16) is independent per key and averages out over the sum, the sum itself stays fp32
+template <typename T>
+__device__ __forceinline__ typename MaVec<T>::v8 ma_pack(const float* x) {
+  typename MaVec<T>::v8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (T)x[i];
+  return r;
+}
+__device__ __forceinline__ constexpr int ma_row(const int r) { return (r & 3) + 8 * (r >> 2); }   // accumulator register -> row (+ 4 * lane half)
+
+// keeps the compiler from carrying x + 0, x + 1, .. x + 31 around a loop in registers of their own
+__device__ __forceinline__ int ma_opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+constexpr float MA_LOG2E = 1.44269504088896340736f, MA_LN2 = 0.69314718055994530942f;
+#define MA_INF __builtin_inff()
+constexpr int MA_KT = 64;          // keys (rows) per tile
+__host__ __device__ inline int ma_tiles(const int n) { return (n + MA_KT - 1) / MA_KT; }
+constexpr int MA_MAX_REACH = 1024; // a head's distance row lives in LDS
+
+// ---- LDS image of a [rows][D] tile: rows of 2 D bytes, 16-byte chunk c of row r at chunk c ^ swz(r).  Two kinds of reads:
+//  * row operand (rows r0 + lane % 32, eight consecutive d): one ds_read_b128, conflict-free (16 rows cover all 64 banks);
+//  * transposed operand (row d = dt * 32 + lane % 32, k = tile rows kb + 4 half + 0..3 and kb + 8 + 4 half + 0..3: the order in which
+//    an accumulator holds its rows): two ds_read_b64_tr_b16, which hand lane i of 16 the four rows of column i of a [4][16] block.
+template <int D>
+struct Tile {
+  static constexpr int RB = 2 * D;
+  static constexpr int CH = D / 8;                       // 16-byte chunks per row
+  __device__ static __forceinline__ int swz(const int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+  __device__ static __forceinline__ int chunk_at(const int row, const int c) { return row * RB + ((c ^ swz(row)) << 4); }
+  // lane's base for row operands; add (r0 * RB), XOR (ks * 32)
+  __device__ static __forceinline__ int row_base(const int lane) { return (lane & 31) * RB + (((lane >> 5) ^ swz(lane & 31)) << 4); }
+  // lane's base for transposed operands
+  __device__ static __forceinline__ int tr_base(const int lane) {
+    const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2), c = ((lane & 31) >> 4) * 2 + ((i & 3) >> 1);
+    return r * RB + ((c ^ swz(r)) << 4) + (i & 1) * 8;
+  }
+  template <typename V8>
+  __device__ static __forceinline__ V8 row_frag(const char* t, const int base, const int r0, const int ks) { return *(const V8*)(t + ((base ^ (ks * 32)) + r0 * RB)); }
+  template <typename V8>
+  __device__ static __forceinline__ V8 tr_frag(const char* t, const int base, const int dt, const int kb) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(ma_lds)(t + ((base ^ (dt * 64)) + kb * RB)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(ma_lds)(t + ((base ^ (dt * 64) ^ (D == 128 ? 128 : 64)) + (kb + 8) * RB)));
+    const s16x8 r = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(V8, r);
+  }
+};
+
+// ---- global -> LDS by DMA (`buffer_load_dwordx4 ... lds`: no staging registers, no ds_write pass).  A piece is 1 KiB of the image = 1024 / RB rows;
+// lane l fills slot l of it and therefore fetches chunk (slot ^ swz(row)) of its row.  An offset past the descriptor's end delivers zeros:
+// rows at or past `limit` (they may hold anything) and chunks past head_dim are sent there.  The base moves with the tile (64-bit), so an
+// offset never passes 31 bits however long the tensor.  The instruction is written as asm so that the compiler does not drain the queue in front of
+// the next LDS read; it has no output register, and the kernel waits (ma_dma_wait) before the barrier that hands the tile over.
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ void ma_dma16(const unsigned lds, const unsigned voff, const uint64_t base) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)base), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(base >> 32)) & 0xffffu,
+                    0x7fffffffu, 0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(voff), "s"(rs) : "memory", "m0");
+}
+// 64 consecutive 4-byte words (one per lane; words at or past `left` arrive as zeros)
+__device__ __forceinline__ void ma_dma4(const unsigned lds, const int lane, const int left, const void* base) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const uint64_t a = (uint64_t)base;
+  const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu,
+                    0x7fffffffu, 0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
+               "v"(lane < left ? lane * 4u : 0x80000000u), "s"(rs) : "memory", "m0");
+}
+#else
+__device__ __forceinline__ void ma_dma16(const unsigned, const unsigned, const uint64_t) {}
+__device__ __forceinline__ void ma_dma4(const unsigned, const int, const int, const void*) {}
+#endif
+__device__ __forceinline__ void ma_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned ma_lds_addr(const void* s) { return (unsigned)(uintptr_t)(ma_lds)s; }
+
+// ROWS x D tile of one matrix, moved by NW waves: this wave's pieces.  With four waves a wave's pieces lie 16 or 32 rows apart, where the swizzle
+// repeats: one lane offset serves all of them and the base moves.
+template <int D, int ROWS, int NW>
+struct TileDma {
+  static constexpr int RPP = 1024 / Tile<D>::RB, NP = ROWS / RPP / NW, STEP = NW * RPP;
+  static constexpr bool SAME = STEP % 16 == 0;
+  unsigned voff[SAME ? 1 : NP];
+  int row0;
+  unsigned lds;             // byte offset of this wave's first piece in the tile
+  __device__ TileDma(const int wave, const int lane, const int64_t stride, const int head_dim) {
+    row0 = wave * RPP + lane / Tile<D>::CH;
+#pragma unroll
+    for (int j = 0; j < (SAME ? 1 : NP); ++j) {
+      const int row = row0 + j * STEP, c = (lane % Tile<D>::CH) ^ Tile<D>::swz(row);
+      voff[j] = c * 8 < head_dim ? (unsigned)(SAME ? row : row0) * (unsigned)(stride * 2) + c * 16 : 0x80000000u;
+    }
+    lds = __builtin_amdgcn_readfirstlane(wave) * 1024;
+  }
+  // the ROWS rows (stride elements apart) that begin first_byte into the matrix at `base` -> the tile at LDS byte address `tile`; rows at or past
+  // `left` and, with `ids` (document numbers of the rows), rows without a document arrive as zeros
+  __device__ __forceinline__ void load(const void* base, const int64_t first_byte, const int64_t stride, const int left, const unsigned tile,
+                                       const int32_t* ids = nullptr) const {
+    const uint64_t a = (uint64_t)base + (uint64_t)first_byte;
+    bool ok[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) ok[j] = row0 + j * STEP < left;
+    if (ids) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) ok[j] = ok[j] && ids[row0 + j * STEP] >= 0;
+    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+      ma_dma16(tile + lds + j * NW * 1024, ok[j] ? voff[SAME ? 0 : j] : 0x80000000u, a + (uint64_t)(stride * (2 * j * STEP)));
+  }
+};
+
+// ---- scores.  A kernel keeps "raw" scores; the score in log2 units is raw * A + B with A > 0, so a softmax probability is one fma and one exp2.
+//  Plain: raw = q.k.   Cap: u = cap tanh(t / cap) = cap (1 - 2 / (1 + e^(2 t / cap))): raw = -1 / (1 + exp2(q.k * pre)), one exp2 and one
+//  reciprocal per score (|error| of u ~ 1e-7 cap).   With a bias: raw is the finished score (A = 1).
+constexpr int MA_CAP = 1, MA_SLOPES = 2, MA_REL = 4;       // MODE bits; slopes and distance rows exclude each other
+template <int MODE>
+struct Score {
+  static constexpr bool CAP = MODE & MA_CAP, SLOPES = MODE & MA_SLOPES, REL = MODE & MA_REL, BIAS = SLOPES || REL;
+  float A, B, pre, capA, slope2;
+  const float* rel;          // LDS: the head's distance row in log2 units
+  int reach;
+  __device__ Score(const MgldMaskAttn& p, const int h, const float* srel) {
+    pre = CAP ? 2.f * MA_LOG2E * p.scale / p.softcap : p.scale * MA_LOG2E;
+    capA = CAP ? 2.f * MA_LOG2E * p.softcap : 0.f;
+    A = BIAS ? 1.f : CAP ? capA : pre;
+    B = CAP && !BIAS ? 0.5f * capA : 0.f;
+    slope2 = SLOPES ? p.slopes[h] * MA_LOG2E : 0.f;
+    rel = srel;
+    reach = p.reach;
+  }
+  __device__ __forceinline__ float squash(const float acc) const { return -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(acc * pre)); }   // in [-1, 0]
+  __device__ __forceinline__ float biased(const float s2, const int delta) const {      // score in log2 units at distance delta = key - query
+    if (SLOPES) return s2 - slope2 * fabsf((float)delta);
+    if (REL) return s2 + rel[min(max(delta, -reach), reach) + reach];
+    return s2;
+  }
+  __device__ __forceinline__ float raw(const float acc, const int delta) const {
+    if (!BIAS) return CAP ? squash(acc) : acc;
+    return biased(CAP ? squash(acc) * capA + 0.5f * capA : acc * pre, delta);
+  }
+  // P = 2^(score - lse2); sq: the squashed dot product, for the cap's derivative
+  __device__ __forceinline__ float prob(const float acc, const int delta, const float lse2, float& sq) const {
+    sq = CAP ? squash(acc) : 0.f;
+    if (!BIAS) return __builtin_amdgcn_exp2f(CAP ? sq * capA + (0.5f * capA - lse2) : acc * pre - lse2);
+    return __builtin_amdgcn_exp2f(biased(CAP ? sq * capA + 0.5f * capA : acc * pre, delta) - lse2);
+  }
+};
+
+// ---- what a batch row lets its queries see
+struct BatchSpan {
+  int len, pos0, prefix;
+  __device__ BatchSpan(const MgldMaskAttn& p, const int b) {
+    len = p.kv_len ? min(max(p.kv_len[b], 0), p.Nkv) : p.Nkv;
+    pos0 = p.q_from_end ? len - p.Nq : p.q_pos0;
+    prefix = p.prefix ? p.prefix[b] : 0;
+  }
+  // keys below this index are in sight of position pos (documents aside)
+  __device__ __forceinline__ int limit(const MgldMaskAttn& p, const int pos) const {
+    return p.causal ? min(len, max(pos < 0x7fffffff ? pos + 1 : pos, prefix)) : len;
+  }
+};
+
+// a group of consecutive query rows [i0, i0 + n): its limits and the range of its document numbers
+struct RowGroup {
+  int lim_min, lim_max;       // smallest / largest limit() over the rows
+  int dmin, dmax;             // over rows with a document; dmin > dmax: none
+  bool uniform;               // every row has the same document
+};
+// documents of rows [i0, i1), reduced over the wave (all lanes call); ids: this batch row's numbers
+__device__ __forceinline__ bool ma_doc_range(const int32_t* ids, const int i0, const int i1, int& dmin, int& dmax, bool& uniform) {
+  int lo = 0x7fffffff, hi = -1, neg = 0;
+  for (int i = i0 + (int)(threadIdx.x & 63); i < i1; i += 64) {
+    const int v = ids[i];
+    if (v >= 0) { lo = min(lo, v); hi = max(hi, v); } else neg = 1;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor(lo, o, 64));
+    hi = max(hi, __shfl_xor(hi, o, 64));
+    neg |= __shfl_xor(neg, o, 64);
+  }
+  dmin = lo; dmax = hi; uniform = !neg && lo == hi;
+  return neg != 0;
+}
+__device__ __forceinline__ RowGroup ma_row_group(const MgldMaskAttn& p, const BatchSpan& bs, const int b, const int i0, const int n) {
+  RowGroup g;
+  const int i1 = min(i0 + n, p.Nq);
+  g.lim_min = bs.limit(p, bs.pos0 + i0);
+  g.lim_max = i1 > i0 ? bs.limit(p, bs.pos0 + i1 - 1) : 0;
+  g.dmin = 0; g.dmax = -1; g.uniform = false;
+  if (p.doc_q) ma_doc_range(p.doc_q + b * p.doc_q_sb, i0, i1, g.dmin, g.dmax, g.uniform);
+  return g;
+}
+
+// document numbers of the 64-row tiles, written by ma_doc_tiles_kernel: {min, max, all 64 rows in one document, some row without}
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+// which tiles of [t0, t0 + 64) the group has to visit (act), and in which of them it sees every pair (full); lane l judges tile t0 + l
+__device__ __forceinline__ void ma_window(const MgldMaskAttn& p, const RowGroup& g, const i32x4 dt, const int t, unsigned long long& act,
+                                          unsigned long long& full) {
+  const int64_t k0 = (int64_t)t * MA_KT;
+  bool a = k0 < g.lim_max, f = k0 + MA_KT <= g.lim_min;
+  if (p.doc_q) {
+    a = a && dt[0] <= g.dmax && dt[1] >= g.dmin;
+    f = f && dt[2] && g.uniform && dt[0] == g.dmin;
+  }
+  act = __ballot(a);
+  full = __ballot(a && f);
+}
+
+// the distance row of head h into LDS, in log2 units (all threads of the block; a barrier follows in the caller)
+__device__ __forceinline__ void ma_load_rel(const MgldMaskAttn& p, const int h, float* srel, const float unit) {
+  const int n = 2 * p.reach + 1;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) srel[i] = p.rel[(int64_t)h * n + i] * unit;
+}
+
+// ---- exact row by row, for the few rows whose fast result is not finite: a product with a zero probability turns an infinity or NaN of a
+// value that the row does not see into NaN.  One wave recomputes row (b, h, i) from its visible keys alone: lanes are keys for the scores,
+// then elements of d for the sum.
+template <typename T>
+__device__ __forceinline__ void ma_slow_row(const MgldMaskAttn& p, const int b, const int h, const int i) {
+  const int lane = threadIdx.x & 63, d = p.head_dim, hk = h / (p.heads / p.kv_heads);
+  const BatchSpan bs(p, b);
+  const int pos = bs.pos0 + i, lim = bs.limit(p, pos);
+  const int dq = p.doc_q ? p.doc_q[b * p.doc_q_sb + i] : 0;
+  const T* q = (const T*)p.Q + b * p.q_sb + (int64_t)i * p.q_si + h * p.q_sh;
+  const T* kb = (const T*)p.K + b * p.k_sb + hk * p.k_sh;
+  const T* vb = (const T*)p.V + b * p.v_sb + hk * p.v_sh;
+  const bool cap = p.softcap > 0.f;
+  auto score = [&](const int j) __attribute__((always_inline)) {          // log2 units; -inf where unseen
+    if (j >= lim || dq < 0 || (p.doc_k && p.doc_k[b * p.doc_k_sb + j] != dq)) return -MA_INF;
+    const T* k = kb + (int64_t)j * p.k_si;
+    float t = 0.f;
+    for (int e = 0; e < d; ++e) t += (float)q[e] * (float)k[e];
+    t *= p.scale;
+    if (cap) t = p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * (2.f * MA_LOG2E / p.softcap))));
+    const int delta = j - pos;
+    if (p.slopes) t -= p.slopes[h] * fabsf((float)delta);
+    if (p.rel) t += p.rel[(int64_t)h * (2 * p.reach + 1) + min(max(delta, -p.reach), p.reach) + p.reach];
+    return t * MA_LOG2E;
+  };
+  auto seen = [&](const int j) __attribute__((always_inline)) { return j < lim && dq >= 0 && !(p.doc_k && p.doc_k[b * p.doc_k_sb + j] != dq); };
+  float m = -MA_INF;
+  for (int j = lane; j < lim; j += 64) m = fmaxf(m, score(j));
+  m = wave_max(m);
+  if (m == -MA_INF) m = 0.f;
+  float l = 0.f, acc0 = 0.f, acc1 = 0.f;
+  for (int j0 = 0; j0 < lim; j0 += 64) {
+    const int j = j0 + lane;
+    const bool s = seen(j);
+    const float pr = s ? __builtin_amdgcn_exp2f(score(j) - m) : 0.f;
+    l += pr;
+    unsigned long long todo = __ballot(s);
+    while (todo) {
+      const int c = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const float pc = __shfl(pr, c, 64);
+      const T* v = vb + (int64_t)(j0 + c) * p.v_si;
+      if (lane < d) acc0 += pc * (float)v[lane];
+      if (lane + 64 < d) acc1 += pc * (float)v[lane + 64];
+    }
+  }
+  l = wave_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
+  if (lane < d) o[lane] = (T)(acc0 * inv);
+  if (lane + 64 < d) o[lane + 64] = (T)(acc1 * inv);
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------------
+// document tiles of keys, then of queries
+inline int64_t ma_doc_bytes(const MgldMaskAttn* p) {
+  return p->doc_q ? ((int64_t)p->batch * (ma_tiles(p->Nkv) + ma_tiles(p->Nq))) * 16 : 0;
+}
+
+}  // namespace
+
+inline int ma_mode(const MgldMaskAttn* p) { return (p->softcap > 0.f ? MA_CAP : 0) | (p->slopes ? MA_SLOPES : 0) | (p->rel ? MA_REL : 0); }
+// calls launch<T, D, MODE>(p, st) for the problem's type, head size and score form
+#define MA_DISPATCH_MODE(launch, T, D, p, st)                                        \
+  switch (ma_mode(p)) {                                                              \
+    case 0: return launch<T, D, 0>(*p, st);                                          \
+    case MA_CAP: return launch<T, D, MA_CAP>(*p, st);                                \
+    case MA_SLOPES: return launch<T, D, MA_SLOPES>(*p, st);                          \
+    case MA_SLOPES | MA_CAP: return launch<T, D, MA_SLOPES | MA_CAP>(*p, st);        \
+    case MA_REL: return launch<T, D, MA_REL>(*p, st);                                \
+    default: return launch<T, D, MA_REL | MA_CAP>(*p, st);                           \
+  }
+#define MA_DISPATCH(launch, p, st)                                                   \
+  if (p->bf16) {                                                                     \
+    if (p->head_dim <= 64) { MA_DISPATCH_MODE(launch, bf16, 64, p, st) }             \
+    MA_DISPATCH_MODE(launch, bf16, 128, p, st)                                       \
+  }                                                                                  \
+  if (p->head_dim <= 64) { MA_DISPATCH_MODE(launch, f16, 64, p, st) }                \
+  MA_DISPATCH_MODE(launch, f16, 128, p, st)
+
+int ma_check(const MgldMaskAttn* p, bool grad);
+int ma_doc_tiles(const MgldMaskAttn& p, void* out, hipStream_t st);

@@ -1,0 +1,574 @@
+// maskattn.hip — attention with capped scores, distance biases and causal / prefix / document / length masks: forward.
+//
+//   s = [softcap tanh(./softcap)](scale q.k) + bias(j - p_i),  o = sum_visible softmax(s) v,  lse = log sum_visible exp s
+//
+// Two kernels: many query rows (one block per 128 rows of a head) and few rows over many keys (keys split over the grid, joined afterwards).
+//  * Scores are computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16): a lane holds 16 keys of ONE query row per 32-key half tile, so the row
+//    maximum and sum are lane-local plus one exchange with lane ^ 32, and the probabilities are the second product's operand as they lie,
+//    O^T = V^T P^T.  V stays row-major in LDS; its transposed fragments come from ds_read_b64_tr_b16.
+//  * One pass with the running maximum (kept in raw units; it moves only when a tile exceeds it by 2^6, so the accumulator is rarely rescaled:
+//    P <= 2^6 fits fp16) and the sum in fp32.
+//  * Which tiles a block visits, and which of them need no mask, is decided 64 tiles at a time: lane l judges tile t0 + l and two
+//    ballots give the bit masks.  A causal, prefix, length or document mask costs skipped tiles nothing and full tiles nothing.
+#include "maskattn.h"
+
+namespace {
+
+// {min, max document number >= 0, all 64 rows in one document, some row without} of each 64-row tile: keys' tiles of every batch row, then the queries'
+__global__ __launch_bounds__(64) void ma_doc_tiles_kernel(const int32_t* dk, const int32_t* dq, const int64_t k_sb, const int64_t q_sb, const int Nkv,
+                                                          const int Nq, const int batch, i32x4* out) {
+  const int ntk = (Nkv + MA_KT - 1) / MA_KT, ntq = (Nq + MA_KT - 1) / MA_KT;
+  const int b = blockIdx.y;
+  int t = blockIdx.x;
+  const bool isq = t >= ntk;
+  if (isq) t -= ntk;
+  const int i0 = t * MA_KT, n = isq ? Nq : Nkv;
+  int lo, hi;
+  bool uni;
+  const bool pad = ma_doc_range(isq ? dq + b * q_sb : dk + b * k_sb, i0, min(i0 + MA_KT, n), lo, hi, uni);
+  if (threadIdx.x == 0) {
+    const i32x4 r = {lo, hi, (int)(uni && i0 + MA_KT <= n), (int)pad};
+    (isq ? out + (int64_t)batch * ntk + (int64_t)b * ntq : out + (int64_t)b * ntk)[t] = r;
+  }
+}
+
+// one 64-key tile of scores -> probabilities packed for the second product; updates the running maximum, sum and accumulators
+template <typename T, int DT, int NH>
+struct RowState {
+  f32x16 o[DT];
+  float m, l;
+  __device__ RowState() : m(-MA_INF), l(0.f) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = ma_zero();
+  }
+  // st: raw scores (masked: -inf); A: log2 units per raw unit; thr: 6 / A.  st becomes the probabilities.
+  __device__ __forceinline__ void step(f32x16 (&st)[NH], const float A, const float thr) {
+    float mx = st[0][0];
+#pragma unroll
+    for (int k2 = 0; k2 < NH; ++k2)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[k2][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    if (__any(mx > m + thr)) {                       // m = -inf: true as soon as something is visible
+      const float mn = mx > m + thr ? mx : m;
+      const float al = m == -MA_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * A);
+      l *= al;
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= al;
+      m = mn;
+    }
+    const float mA = m == -MA_INF ? 0.f : m * A;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k2 = 0; k2 < NH; ++k2)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        st[k2][r] = __builtin_amdgcn_exp2f(st[k2][r] * A - mA);
+        st[k2][r + 1] = __builtin_amdgcn_exp2f(st[k2][r + 1] * A - mA);
+        s0 += st[k2][r];
+        s1 += st[k2][r + 1];
+      }
+    l += s0 + s1;
+  }
+};
+
+// masks a 32-key half of raw scores: keys k0 + ma_row(r) + 4 half at or past `lim`, or of another document than dq
+template <bool DOCS>
+__device__ __forceinline__ void ma_mask(f32x16& st, const int k0, const int lhi, const int lim, const int* sdoc, const int dq) {
+  const int left = ma_opaque(lim - k0 - lhi * 4);
+#pragma unroll
+  for (int rg = 0; rg < 4; ++rg) {                     // registers 4 rg .. + 3: four consecutive keys
+    const int j = rg * 8 + lhi * 4;
+    i32x4 dk = {dq, dq, dq, dq};
+    if (DOCS) dk = *(const i32x4*)(sdoc + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool vis = (rg * 8 + e < left) & (dk[e] == dq);
+      st[rg * 4 + e] = vis ? st[rg * 4 + e] : -MA_INF;
+    }
+  }
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------------------------------------
+// block: 4 waves x 32 query rows of one head; K / V tiles of 64 keys go by DMA into two LDS buffers (tile t + 1 is on its way while tile t
+// feeds the matrix cores), one barrier per tile.
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const MgldMaskAttn p, const i32x4* __restrict__ kdoc, const int nqb) {
+  typedef typename MaVec<T>::v8 v8;
+  typedef Tile<D> TL;
+  constexpr int DK = D / 16, DT = D / 32;
+  constexpr int TBYTES = MA_KT * TL::RB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];              // [2] x {K, V}, then doc numbers [2][64], then the distance row
+  int* const sdoc = (int*)(smem + 4 * TBYTES);
+  float* const srel = (float*)(sdoc + 2 * MA_KT);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lhi = lane >> 5;
+
+  // block -> (batch row, head, row block).  Blocks go round-robin to the 8 XCDs: XCD x takes consecutive heads (which share K and V, and the L2),
+  // all of them at one row block before the next; the last row blocks (the longest under a causal mask) come first.
+  const int nbh = p.batch * p.heads;
+  int bh, qb;
+  if (nbh % 8 == 0) {
+    const int per = nbh / 8, x = blockIdx.x & 7, j = blockIdx.x >> 3;
+    bh = x * per + j % per;
+    qb = nqb - 1 - j / per;
+  } else {
+    bh = blockIdx.x % nbh;
+    qb = nqb - 1 - blockIdx.x / nbh;
+  }
+  const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kv_heads);
+  const int i0 = qb * 128, iw = i0 + wave * 32;
+  const BatchSpan bs(p, b);
+  const RowGroup gb = ma_row_group(p, bs, b, i0, 128), gw = ma_row_group(p, bs, b, iw, 32);
+  const bool docs = p.doc_q != nullptr;
+  const int ntk = (p.Nkv + MA_KT - 1) / MA_KT;
+  if (docs) kdoc += (int64_t)b * ntk;
+
+  const T* __restrict__ Qp = (const T*)p.Q + b * p.q_sb + h * p.q_sh;
+  const T* __restrict__ Kp = (const T*)p.K + b * p.k_sb + hk * p.k_sh;
+  const T* __restrict__ Vp = (const T*)p.V + b * p.v_sb + hk * p.v_sh;
+  const int d8 = p.head_dim / 8;
+  v8 zero;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) zero[i] = (T)0.f;
+
+  const int i = iw + l31;
+  const int pos = bs.pos0 + i;
+  const int lim = i < p.Nq ? bs.limit(p, pos) : 0;
+  const int dq = docs && i < p.Nq ? p.doc_q[b * p.doc_q_sb + i] : -1;
+  const int dqm = dq < 0 ? -2 : dq;                    // a row without document equals no key's number
+  v8 qf[DK];
+#pragma unroll
+  for (int ks = 0; ks < DK; ++ks) qf[ks] = i < p.Nq && ks * 2 + lhi < d8 ? *(const v8*)(Qp + (int64_t)i * p.q_si + ks * 16 + lhi * 8) : zero;
+  if (MODE & MA_REL) ma_load_rel(p, h, srel, MA_LOG2E);
+  const Score<MODE> sc(p, h, srel);
+  const float thr = 6.f / sc.A;
+
+  // tiles to visit
+  const int nt = ma_tiles(gb.lim_max);
+  int w0 = -64;
+  unsigned long long bact = 0, wact = 0, wfull = 0, bfull = 0, pads = 0;
+  auto advance = [&](int& flags) __attribute__((always_inline)) {      // next tile of the block, or -1; flags: 1 the wave visits it, 2 without mask, 4 padding rows
+    while (!bact) {
+      w0 += 64;
+      if (w0 >= nt) return -1;
+      const i32x4 dt = docs && w0 + lane < ntk ? kdoc[w0 + lane] : i32x4{0x7fffffff, -1, 0, 0};
+      ma_window(p, gb, dt, w0 + lane, bact, bfull);
+      ma_window(p, gw, dt, w0 + lane, wact, wfull);
+      pads = __ballot(dt[3] != 0);
+    }
+    const int c = __builtin_ctzll(bact);
+    bact &= bact - 1;
+    flags = (int)((wact >> c) & 1) | (int)((wfull >> c) & 1) << 1 | (int)((pads >> c) & 1) << 2;
+    return w0 + c;
+  };
+
+  // tile t -> buffer `buf`
+  const TileDma<D, MA_KT, 4> dk(wave, lane, p.k_si, p.head_dim), dv(wave, lane, p.v_si, p.head_dim);
+  const unsigned lds0 = ma_lds_addr(smem);
+  auto load_tile = [&](const int t, const int buf, const int flags) __attribute__((always_inline)) {
+    const int k0 = t * MA_KT;
+    const unsigned a = lds0 + buf * 2 * TBYTES;
+    const int32_t* const ids = docs ? p.doc_k + b * p.doc_k_sb + k0 : nullptr;
+    dk.load(Kp, (int64_t)k0 * p.k_si * 2, p.k_si, bs.len - k0, a, flags & 4 ? ids : nullptr);
+    dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, bs.len - k0, a + TBYTES, flags & 4 ? ids : nullptr);
+    if (docs && wave == 0) ma_dma4(lds0 + 4 * TBYTES + buf * MA_KT * 4, lane, bs.len - k0, ids);      // (zeros past the length: `lim` hides them)
+  };
+
+  RowState<T, DT, 2> rs;
+  const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
+  int fl = 0, fln = 0;
+  int t = advance(fl), buf = 0;
+  if (t >= 0) load_tile(t, 0, fl);
+  while (t >= 0) {
+    ma_dma_wait();
+    __syncthreads();                                   // tile t has landed everywhere, and everyone is done with the other buffer
+    const int tn = advance(fln);
+    if (tn >= 0) load_tile(tn, buf ^ 1, fln);
+    if (fl & 1) {
+      const char* const sk = smem + buf * 2 * TBYTES;
+      const char* const sv = sk + TBYTES;
+      f32x16 st[2];
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        __builtin_amdgcn_sched_barrier(0);
+        st[k2] = ma_zero();
+#pragma unroll
+        for (int ks = 0; ks < DK; ++ks) st[k2] = ma_mfma(TL::template row_frag<v8>(sk, kbase, k2 * 32, ks), qf[ks], st[k2]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const int k0 = t * MA_KT;
+      if (MODE) {
+        const int dl = ma_opaque(k0 + 4 * lhi - pos);
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[k2][r] = sc.raw(st[k2][r], dl + k2 * 32 + ma_row(r));
+      }
+      if (!(fl & 2)) {
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+          if (docs) ma_mask<true>(st[k2], k0 + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dqm);
+          else ma_mask<false>(st[k2], k0 + k2 * 32, lhi, lim, nullptr, 0);
+        }
+      }
+      rs.step(st, sc.A, thr);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        __builtin_amdgcn_sched_barrier(0);            // fragment reads stay beside their products (registers)
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = st[s >> 1][(s & 1) * 8 + e];
+        const v8 pf = ma_pack<T>(x);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) rs.o[dt] = ma_mfma(TL::template tr_frag<v8>(sv, vbase, dt, s * 16), pf, rs.o[dt]);
+      }
+    }
+    buf ^= 1;
+    t = tn; fl = fln;
+  }
+
+  // ---- epilogue: O[i][d] = O^T[d][i] / l
+  const float l = rs.l + __shfl_xor(rs.l, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float z = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z += rs.o[dt][r] * 0.f;
+  const unsigned long long bz = __ballot(z != z);      // an infinity or NaN came in
+  unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
+  if (i < p.Nq) {
+    if (p.lse && lhi == 0) p.lse[((int64_t)b * p.heads + h) * p.Nq + i] = l == 0.f ? -MA_INF : (rs.m * sc.A + sc.B + __builtin_amdgcn_logf(l)) * MA_LN2;
+    if (!((bad >> l31) & 1)) {
+      T* const o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int rg = 0; rg < 4; ++rg) {
+          const int d = dt * 32 + rg * 8 + lhi * 4;
+          typedef T t4 __attribute__((ext_vector_type(4)));
+          if (d < p.head_dim)
+            *(t4*)(o + d) = t4{(T)(rs.o[dt][rg * 4] * inv), (T)(rs.o[dt][rg * 4 + 1] * inv), (T)(rs.o[dt][rg * 4 + 2] * inv), (T)(rs.o[dt][rg * 4 + 3] * inv)};
+        }
+    }
+  }
+  while (bad) {
+    const int r = __builtin_ctz(bad);
+    bad &= bad - 1;
+    if (iw + r < p.Nq) ma_slow_row<T>(p, b, h, iw + r);
+  }
+}
+
+// ---- few rows over many keys ----------------------------------------------------------------------------------------------------------
+// Rows of the query heads that share a key head are packed: packed row r = (query i = r / G, head of the group g = r % G); a block takes 32 of
+// them and one slice of the tiles, its 4 waves every fourth tile each, by DMA into LDS of their own (no barrier in the loop).  The waves' states
+// meet in LDS, the slices' in ma_join_kernel through fp32 partial results in the work buffer.
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, const i32x4* __restrict__ kdoc, const int nsplit, const int nrb, float* part) {
+  typedef typename MaVec<T>::v8 v8;
+  typedef Tile<D> TL;
+  constexpr int DK = D / 16, DT = D / 32, KH = 32;
+  constexpr int TBYTES = KH * TL::RB;
+  extern __shared__ __attribute__((aligned(16))) char smem[];              // per wave [2] x {K, V} of 32 keys (later: its O [32][D] fp32), doc numbers, m / l, distance rows
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lhi = lane >> 5;
+  int* const sdoc = (int*)(smem + 16 * TBYTES) + wave * 2 * MA_KT;         // (a DMA writes 64 words)
+  float* const sml = (float*)(smem + 16 * TBYTES) + 8 * MA_KT;             // [4][2][32]
+  float* const srel = sml + 256;
+  const int G = p.heads / p.kv_heads, rows = G * p.Nq;
+  const int split = blockIdx.x, hk = blockIdx.y % p.kv_heads, rb = blockIdx.y / p.kv_heads, b = blockIdx.z;
+  const BatchSpan bs(p, b);
+  const bool docs = p.doc_q != nullptr;
+  const int ntk = (p.Nkv + MA_KT - 1) / MA_KT;
+  if (docs) kdoc += (int64_t)b * ntk;
+
+  const int r = rb * 32 + l31;
+  const bool rok = r < rows;
+  const int i = rok ? r / G : 0, h = hk * G + (rok ? r % G : 0), pos = bs.pos0 + i;
+  const int lim = rok ? bs.limit(p, pos) : 0;
+  const int dq = docs && rok ? p.doc_q[b * p.doc_q_sb + i] : -1, dqm = dq < 0 ? -2 : dq;
+  const int if_ = rb * 32 / G, il = (min(rb * 32 + 32, rows) - 1) / G;     // queries of this block
+  const RowGroup g = ma_row_group(p, bs, b, if_, il - if_ + 1);
+  const T* __restrict__ Kp = (const T*)p.K + b * p.k_sb + hk * p.k_sh;
+  const T* __restrict__ Vp = (const T*)p.V + b * p.v_sb + hk * p.v_sh;
+  const int d8 = p.head_dim / 8;
+  v8 zero;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) zero[e] = (T)0.f;
+  v8 qf[DK];
+  {
+    const T* q = (const T*)p.Q + b * p.q_sb + (int64_t)i * p.q_si + h * p.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) qf[ks] = rok && ks * 2 + lhi < d8 ? *(const v8*)(q + ks * 16 + lhi * 8) : zero;
+  }
+  // a lane's head differs from its neighbour's: the distance rows of the group's heads lie side by side
+  if (MODE & MA_REL) {
+    const int n = 2 * p.reach + 1;
+    for (int e = tid; e < G * n; e += 256) srel[e] = p.rel[(int64_t)hk * G * n + e] * MA_LOG2E;
+  }
+  __syncthreads();
+  const Score<MODE> sc(p, h, srel + (rok ? r % G : 0) * (2 * p.reach + 1));
+  const float thr = 6.f / sc.A;
+
+  // this block's tiles: an equal share of those below the rows' limits
+  const int nt = ma_tiles(g.lim_max), share = (nt + nsplit - 1) / nsplit;
+  const int ta = min(split * share, nt), tb = min(ta + share, nt);
+  int w0 = ta - 64;
+  unsigned long long act = 0, full = 0;
+  int cur = -1, half = 1, curfull = 0;
+  auto advance = [&](int& fullf) __attribute__((always_inline)) {      // next 32-key half tile, or -1
+    if (half == 0 && (cur * 2 + 1) * KH < g.lim_max) { half = 1; fullf = curfull; return cur * 2 + 1; }
+    while (!act) {
+      w0 += 64;
+      if (w0 >= tb) return -1;
+      const int t = w0 + lane;
+      const i32x4 dt = docs && t < ntk ? kdoc[t] : i32x4{0x7fffffff, -1, 0, 0};
+      ma_window(p, g, dt, t, act, full);
+      act &= __ballot(t < tb && ((t - ta) & 3) == wave);
+    }
+    const int c = __builtin_ctzll(act);
+    act &= act - 1;
+    cur = w0 + c; half = 0; curfull = (int)((full >> c) & 1);
+    fullf = curfull;
+    return cur * 2;
+  };
+
+  const TileDma<D, KH, 1> dk(0, lane, p.k_si, p.head_dim), dv(0, lane, p.v_si, p.head_dim);
+  const unsigned lds0 = ma_lds_addr(smem) + __builtin_amdgcn_readfirstlane(wave) * 4 * TBYTES;
+  const unsigned lds_doc = ma_lds_addr(smem) + 16 * TBYTES + __builtin_amdgcn_readfirstlane(wave) * 2 * MA_KT * 4;
+  auto load_half = [&](const int t, const int buf) __attribute__((always_inline)) {
+    const int k0 = t * KH;
+    const unsigned a = lds0 + buf * 2 * TBYTES;
+    dk.load(Kp, (int64_t)k0 * p.k_si * 2, p.k_si, g.lim_max - k0, a);
+    dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, g.lim_max - k0, a + TBYTES);
+    if (docs) ma_dma4(lds_doc + buf * MA_KT * 4, lane, min(KH, g.lim_max - k0), p.doc_k + b * p.doc_k_sb + k0);
+  };
+  RowState<T, DT, 1> rs;
+  const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
+  int fl = 0, buf = 0;
+  int t = advance(fl);
+  if (t >= 0) load_half(t, 0);
+  while (t >= 0) {
+    ma_dma_wait();                                       // the wave's own tile: no other wave reads it
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int fln = 0;
+    const int tn = advance(fln);
+    if (tn >= 0) load_half(tn, buf ^ 1);
+    const char* const sk = smem + wave * 4 * TBYTES + buf * 2 * TBYTES;
+    const char* const sv = sk + TBYTES;
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 st[1];
+    st[0] = ma_zero();
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) st[0] = ma_mfma(TL::template row_frag<v8>(sk, kbase, 0, ks), qf[ks], st[0]);
+    const int k0 = t * KH;
+    if (MODE) {
+      const int dl = ma_opaque(k0 + 4 * lhi - pos);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st[0][e] = sc.raw(st[0][e], dl + ma_row(e));
+    }
+    if (!fl) {
+      if (docs) ma_mask<true>(st[0], k0, lhi, lim, sdoc + buf * MA_KT, dqm);
+      else ma_mask<false>(st[0], k0, lhi, lim, nullptr, 0);
+    }
+    rs.step(st, sc.A, thr);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      __builtin_amdgcn_sched_barrier(0);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = st[0][s * 8 + e];
+      const v8 pf = ma_pack<T>(x);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) rs.o[dt] = ma_mfma(TL::template tr_frag<v8>(sv, vbase, dt, s * 16), pf, rs.o[dt]);
+    }
+    t = tn; fl = fln; buf ^= 1;
+  }
+
+  // ---- the four waves' states meet: o * 2^((m_w - M) A)
+  const float l = rs.l + __shfl_xor(rs.l, 32, 64);
+  __syncthreads();                                       // every wave is done with its tiles
+  if (lhi == 0) { sml[wave * 64 + l31] = rs.m; sml[wave * 64 + 32 + l31] = l; }
+  float* const so = (float*)smem + wave * 32 * D;        // [32 rows][D] fp32 = the wave's two tiles' bytes
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg)
+      *(f32x4*)(so + l31 * D + ((dt * 32 + rg * 8 + lhi * 4) ^ ((l31 & 7) * 4))) =
+          f32x4{rs.o[dt][rg * 4], rs.o[dt][rg * 4 + 1], rs.o[dt][rg * 4 + 2], rs.o[dt][rg * 4 + 3]};
+  __syncthreads();
+  for (int rr = wave; rr < 32; rr += 4) {                // a wave per row, lanes over d
+    const int pr = rb * 32 + rr;
+    if (pr >= rows) break;
+    float M = -MA_INF;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, sml[w * 64 + rr]);
+    float L = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = sml[w * 64 + rr];
+      const float f = mw == -MA_INF ? 0.f : __builtin_amdgcn_exp2f((mw - M) * sc.A);
+      L += sml[w * 64 + 32 + rr] * f;
+      const float* ow = (const float*)smem + w * 32 * D + rr * D;
+      a0 += ow[lane ^ ((rr & 7) * 4)] * f;
+      if (D == 128) a1 += ow[(lane + 64) ^ ((rr & 7) * 4)] * f;
+    }
+    const int ii = pr / G, hh = hk * G + pr % G;
+    if (nsplit > 1) {
+      const int64_t slot = (((int64_t)b * p.heads + hh) * p.Nq + ii) * nsplit + split;
+      float* const po = part + slot * (D + 2);
+      po[lane] = a0;
+      if (D == 128) po[lane + 64] = a1;
+      if (lane == 0) { po[D] = M * sc.A + sc.B; po[D + 1] = L; }           // the maximum in log2 units
+    } else {
+      const bool bad = __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f);
+      if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + hh) * p.Nq + ii] = L == 0.f ? -MA_INF : (M * sc.A + sc.B + __builtin_amdgcn_logf(L)) * MA_LN2;
+      if (bad) ma_slow_row<T>(p, b, hh, ii);
+      else {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        T* const o = (T*)p.O + b * p.o_sb + (int64_t)ii * p.o_si + hh * p.o_sh;
+        if (lane < p.head_dim) o[lane] = (T)(a0 * inv);
+        if (lane + 64 < p.head_dim) o[lane + 64] = (T)(a1 * inv);
+      }
+    }
+  }
+}
+
+// joins the slices of one row: a wave per row
+template <typename T, int D>
+__global__ __launch_bounds__(64) void ma_join_kernel(const MgldMaskAttn p, const float* part, const int nsplit) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float* const po = part + row * nsplit * (D + 2);
+  float M = -MA_INF;
+  for (int s = lane; s < nsplit; s += 64) M = fmaxf(M, po[(int64_t)s * (D + 2) + D]);
+  M = wave_max(M);
+  float L = 0.f, a0 = 0.f, a1 = 0.f;
+  for (int s = 0; s < nsplit; ++s) {
+    const float* const ps = po + (int64_t)s * (D + 2);
+    const float f = ps[D] == -MA_INF ? 0.f : __builtin_amdgcn_exp2f(ps[D] - M);
+    L += ps[D + 1] * f;
+    a0 += ps[lane] * f;
+    if (D == 128) a1 += ps[lane + 64] * f;
+  }
+  const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.heads), b = (int)(row / p.Nq / p.heads);
+  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -MA_INF : (M + __builtin_amdgcn_logf(L)) * MA_LN2;
+  if (__any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f)) {
+    ma_slow_row<T>(p, b, h, i);
+    return;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* const o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
+  if (lane < p.head_dim) o[lane] = (T)(a0 * inv);
+  if (lane + 64 < p.head_dim) o[lane + 64] = (T)(a1 * inv);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+int ma_cus() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+  return n;
+}
+
+struct Plan { bool split; int nsplit, nrb; };
+// few rows: when one block per 128 rows would leave most of the card idle and there are keys to share out
+Plan ma_plan(const MgldMaskAttn* p) {
+  Plan pl{false, 1, 1};
+  const int G = p->heads / p->kv_heads, nt = ma_tiles(p->Nkv);
+  const int64_t rows = (int64_t)G * p->Nq;
+  const int64_t blocks = (int64_t)p->batch * p->heads * ((p->Nq + 127) / 128);
+  const int64_t packed = (int64_t)p->batch * p->kv_heads * ((rows + 31) / 32);
+  const bool rel_fits = !p->rel || (int64_t)G * (2 * p->reach + 1) * 4 <= 28 * 1024;       // (beside 131 KB of tiles)
+  pl.split = rel_fits && (rows + 31) / 32 * p->kv_heads <= 65535 && p->batch <= 65535 && (p->Nq <= 16 || (blocks * 4 <= 256 && nt >= 16));
+  if (!pl.split) return pl;
+  pl.nrb = (int)((rows + 31) / 32);
+  // two blocks per CU; a slice keeps at least one tile for each of its four waves
+  int64_t n = (2 * 256 + packed - 1) / packed;
+  if (n > (nt + 3) / 4) n = (nt + 3) / 4;
+  if (n > 128) n = 128;
+  pl.nsplit = n < 1 ? 1 : (int)n;
+  return pl;
+}
+
+template <typename T, int D, int MODE>
+int ma_launch(const MgldMaskAttn& p, hipStream_t st) {
+  const Plan pl = ma_plan(&p);
+  const i32x4* kdoc = (const i32x4*)p.work;
+  float* part = (float*)((char*)p.work + ma_doc_bytes(&p));
+  const int nrel = p.rel ? 2 * p.reach + 1 : 0;
+  if (p.doc_q) {
+    const int rc = ma_doc_tiles(p, p.work, st);
+    if (rc) return rc;
+  }
+  if (!pl.split) {
+    const int64_t nqb = (p.Nq + 127) / 128, nb = nqb * p.batch * p.heads;
+    MGLD_REQUIRE(nb <= 0x7fffffff, "masked_attention: grid");
+    const int lds = 4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + nrel * 4;
+    static_assert(4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + (2 * MA_MAX_REACH + 1) * 4 <= 80 * 1024, "two blocks per CU");
+    if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)ma_fwd_kernel<T, D, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    ma_fwd_kernel<T, D, MODE><<<dim3((unsigned)nb), 256, lds, st>>>(p, kdoc, (int)nqb);
+    return mgld_check_launch("masked_attention");
+  }
+  const int G = p.heads / p.kv_heads;
+  const int lds = 16 * 32 * Tile<D>::RB + 8 * MA_KT * 4 + 256 * 4 + G * nrel * 4;
+  if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)ma_split_kernel<T, D, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  ma_split_kernel<T, D, MODE><<<dim3(pl.nsplit, pl.nrb * p.kv_heads, p.batch), 256, lds, st>>>(p, kdoc, pl.nsplit, pl.nrb, part);
+  if (pl.nsplit > 1) ma_join_kernel<T, D><<<dim3((unsigned)((int64_t)p.batch * p.heads * p.Nq)), 64, 0, st>>>(p, part, pl.nsplit);
+  return mgld_check_launch("masked_attention");
+}
+bool ma_aligned(const void* ptr, const int64_t sb, const int64_t si, const int64_t sh) {
+  return ptr && (uintptr_t)ptr % 16 == 0 && sb % 8 == 0 && si % 8 == 0 && sh % 8 == 0;
+}
+
+}  // namespace
+
+int ma_check(const MgldMaskAttn* p, const bool grad) {
+  MGLD_REQUIRE(p && p->batch >= 0 && p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0, "masked_attention: heads must be a multiple of kv_heads");
+  MGLD_REQUIRE(p->Nq >= 0 && p->Nkv >= 0 && p->Nq <= (1 << 30) && p->Nkv <= (1 << 30), "masked_attention: lengths");
+  MGLD_REQUIRE(p->head_dim >= 8 && p->head_dim <= 128 && p->head_dim % 8 == 0, "masked_attention: head_dim must be a multiple of 8 up to 128");
+  MGLD_REQUIRE(p->scale > 0.f && p->scale < 3e38f && p->softcap >= 0.f && p->softcap < 3e38f, "masked_attention: scale > 0, softcap >= 0");
+  MGLD_REQUIRE(p->q_pos0 >= -(1 << 30) && p->q_pos0 <= (1 << 30) , "masked_attention: q_pos0");
+  MGLD_REQUIRE(!p->rel || (p->reach >= 0 && p->reach <= MA_MAX_REACH), "masked_attention: reach up to 1024");
+  MGLD_REQUIRE(!p->rel || !p->slopes, "masked_attention: slopes or rel, not both");
+  MGLD_REQUIRE(!grad || !p->rel || (int64_t)(p->heads / p->kv_heads) * (2 * p->reach + 1) * 4 <= 92 * 1024,
+               "masked_attention_grad: the distance rows of the query heads that share a key head must fit 92 KB");
+  MGLD_REQUIRE(!p->prefix || p->causal, "masked_attention: prefix needs causal");
+  MGLD_REQUIRE((p->doc_q != nullptr) == (p->doc_k != nullptr) || p->Nq == 0 || p->Nkv == 0, "masked_attention: doc_q and doc_k go together");
+  if (p->batch == 0 || (p->Nq == 0 && !grad)) return MGLD_OK;
+  if (p->Nq > 0) {
+    MGLD_REQUIRE(ma_aligned(p->Q, p->q_sb, p->q_si, p->q_sh) && ma_aligned(p->O, p->o_sb, p->o_si, p->o_sh), "masked_attention: q / o must be 16-byte aligned with strides of multiples of 8");
+    if (grad) MGLD_REQUIRE(ma_aligned(p->dO, p->do_sb, p->do_si, p->do_sh) && ma_aligned(p->dQ, p->dq_sb, p->dq_si, p->dq_sh) && p->lse, "masked_attention_grad: do / dq alignment, lse");
+  }
+  // a tile's rows are addressed with 31-bit byte offsets (its base with 64 bits)
+  auto row_ok = [](const int64_t si) { return si >= 0 && si < (1 << 23); };
+  MGLD_REQUIRE(row_ok(p->q_si) && row_ok(p->k_si) && row_ok(p->v_si) && (!grad || row_ok(p->do_si)), "masked_attention: row strides must be below 2^23 elements");
+  if (p->Nkv > 0) {
+    MGLD_REQUIRE(ma_aligned(p->K, p->k_sb, p->k_si, p->k_sh) && ma_aligned(p->V, p->v_sb, p->v_si, p->v_sh), "masked_attention: k / v must be 16-byte aligned with strides of multiples of 8");
+    if (grad) MGLD_REQUIRE(ma_aligned(p->dK, p->dk_sb, p->dk_si, p->dk_sh) && ma_aligned(p->dV, p->dv_sb, p->dv_si, p->dv_sh), "masked_attention_grad: dk / dv alignment");
+  }
+  return MGLD_OK;
+}
+
+int ma_doc_tiles(const MgldMaskAttn& p, void* out, hipStream_t st) {
+  MGLD_REQUIRE(p.batch <= 65535, "masked_attention: batch with documents up to 65535");
+  const int n = ma_tiles(p.Nkv) + ma_tiles(p.Nq);
+  if (n > 0) ma_doc_tiles_kernel<<<dim3(n, p.batch), 64, 0, st>>>(p.doc_k, p.doc_q, p.doc_k_sb, p.doc_q_sb, p.Nkv, p.Nq, p.batch, (i32x4*)out);
+  return mgld_check_launch("masked_attention documents");
+}
+
+extern "C" int64_t mgld_masked_attention_work(const MgldMaskAttn* p) {
+  if (!p || ma_check(p, false) || p->batch == 0 || p->Nq == 0) return 0;
+  const Plan pl = ma_plan(p);
+  const int D = p->head_dim <= 64 ? 64 : 128;
+  return ma_doc_bytes(p) + (pl.nsplit > 1 ? (int64_t)p->batch * p->heads * p->Nq * pl.nsplit * (D + 2) * 4 : 0);
+}
+
+extern "C" int mgld_masked_attention(const MgldMaskAttn* p, void* stream) {
+  const int rc = ma_check(p, false);
+  if (rc || p->batch == 0 || p->Nq == 0) return rc;
+  const int64_t need = mgld_masked_attention_work(p);
+  MGLD_REQUIRE(need == 0 || (p->work && (uintptr_t)p->work % 16 == 0 && p->work_bytes >= need), "masked_attention: work buffer too small");
+  hipStream_t st = (hipStream_t)stream;
+  MA_DISPATCH(ma_launch, p, st)
+}

@@ -1,0 +1,335 @@
+// qkrope.hip — root-mean-square norm of every query / key head and the position rotation, one pass over the two projections, and its gradient.
+//
+//   n = x r g,  r = (mean_d x^2 + eps)^-1/2;   pair (a, b) of n at position p:  (a cos - b sin, a sin + b cos),  angle = p freqs[j]
+//   gradient: z = R^T dy,  dg = sum_{rows, heads} z x r,  dx = r (g z - x r mean_d(g z x r))
+//
+// Bound: HBM (forward 4 bytes per element, gradient 6); everything a head needs sits in the registers of one group of lanes.
+//  * A lane holds P = 8 pairs (two 16-byte loads; P = 4 / 8-byte loads where sizes or alignment ask for it), a head is a group of
+//    d / 2P lanes padded to a power of two, so the sum of squares is log2(group) exchanges and no LDS.
+//  * A group keeps ONE token and walks over heads: the P sines and cosines of its pairs are computed once and stay in registers.
+//    The angle is reduced in fp64 (turns = p * freqs / 2 pi minus its nearest integer: 2^-31 of a turn at p = 2^20, where an fp32 product is
+//    off by 2^-4), then sincospi in fp32.  Each sine is needed by one group per block, so nothing is tabulated.
+//  * dg is summed in fp32 inside a block (a lane over its tokens and heads, then the groups in order) and in fp64 over the blocks, in a
+//    fixed order: the same call gives the same bits.
+#include "common.h"
+
+namespace {
+
+typedef __bf16 bf16;
+template <typename T, int N> struct qr_vec { typedef T type __attribute__((ext_vector_type(N))); };
+
+// P pairs of a head as this lane holds them: (a[i], b[i]); element indices of the two halves it loads
+template <int P, bool IL>
+struct PairMap {
+  int e0, e1;        // first element of the lane's two P-element vectors
+  bool rot, on;
+  int j0;            // first pair (index into freqs) when rot
+  __device__ PairMap(const int slot, const int d, const int rd) {
+    const int p = slot * P;
+    on = 2 * p < d;
+    rot = 2 * p < rd;
+    j0 = p;
+    if (IL) { e0 = 2 * p; e1 = 2 * p + P; }
+    else if (rot) { e0 = p; e1 = rd / 2 + p; }
+    else { e0 = rd + (p - rd / 2); e1 = e0 + (d - rd) / 2; }
+  }
+};
+
+template <typename T, int P, bool IL>
+__device__ __forceinline__ void load_pairs(const T* x, const PairMap<P, IL>& m, float (&a)[P], float (&b)[P]) {
+  typedef typename qr_vec<T, P>::type V;
+  const V u = *(const V*)(x + m.e0), v = *(const V*)(x + m.e1);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (IL) {
+      a[i] = (float)(2 * i < P ? u[(2 * i) % P] : v[(2 * i) % P]);
+      b[i] = (float)(2 * i < P ? u[(2 * i + 1) % P] : v[(2 * i + 1) % P]);
+    } else {
+      a[i] = (float)u[i];
+      b[i] = (float)v[i];
+    }
+  }
+}
+template <typename T, int P, bool IL>
+__device__ __forceinline__ void store_pairs(T* y, const PairMap<P, IL>& m, const float (&a)[P], const float (&b)[P]) {
+  typedef typename qr_vec<T, P>::type V;
+  V u, v;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (IL) {
+      if (2 * i < P) { u[(2 * i) % P] = (T)a[i]; u[(2 * i + 1) % P] = (T)b[i]; }
+      else { v[(2 * i) % P] = (T)a[i]; v[(2 * i + 1) % P] = (T)b[i]; }
+    } else {
+      u[i] = (T)a[i];
+      v[i] = (T)b[i];
+    }
+  }
+  *(V*)(y + m.e0) = u;
+  *(V*)(y + m.e1) = v;
+}
+template <int P, bool IL>
+__device__ __forceinline__ void load_gamma(const float* g, const PairMap<P, IL>& m, float (&a)[P], float (&b)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int ea = IL ? m.e0 + 2 * i : m.e0 + i, eb = IL ? m.e0 + 2 * i + 1 : m.e1 + i;
+    a[i] = g && m.on ? g[ea] : 1.f;
+    b[i] = g && m.on ? g[eb] : 1.f;
+  }
+}
+template <int P, bool IL>
+__device__ __forceinline__ void turn_of(const MgldQkRope& p, const int64_t row, const PairMap<P, IL>& m, float (&c)[P], float (&s)[P]) {
+  const double pos = p.rot_dim == 0 ? 0. : p.pos64 ? (double)((const int64_t*)p.pos)[row] : (double)((const int32_t*)p.pos)[row];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+    if (m.on && m.rot) {
+      double t = pos * (p.freqs[m.j0 + i] * 0.15915494309189533577);
+      t -= rint(t);
+      sincospif(2.f * (float)t, &s[i], &c[i]);
+    }
+  }
+}
+template <int LG>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LG / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// one block: TB = 256 / (LG * GT) tokens, GT groups per token; a group takes heads h = its index, + GT, ...
+template <typename T, int P, int LG, bool IL>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, const int GT) {
+  const int grp = threadIdx.x / LG, slot = threadIdx.x % LG;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LG / GT) + grp / GT;
+  if (row >= p.rows) return;
+  const PairMap<P, IL> m(slot, p.head_dim, p.rot_dim);
+  const float inv_d = 1.f / (float)p.head_dim;
+  const int first = (int)blockIdx.y * GT + grp % GT, step = GT * (int)gridDim.y, H = p.q.heads + p.k.heads;
+  auto src = [&](const int h) __attribute__((always_inline)) {
+    return h < p.q.heads ? (const T*)p.q.x + row * p.q.x_sr + (int64_t)h * p.q.x_sh
+                         : (const T*)p.k.x + row * p.k.x_sr + (int64_t)(h - p.q.heads) * p.k.x_sh;
+  };
+  float c[P], s[P], gqa[P], gqb[P], gka[P], gkb[P], a[P], b[P];
+  if (first < H && m.on) load_pairs<T, P, IL>(src(first), m, a, b);
+  turn_of<P, IL>(p, row, m, c, s);
+  load_gamma<P, IL>(p.q.gamma, m, gqa, gqb);
+  load_gamma<P, IL>(p.k.gamma, m, gka, gkb);
+  for (int h = first; h < H; h += step) {
+    float na[P], nb[P];
+    if (h + step < H && m.on) load_pairs<T, P, IL>(src(h + step), m, na, nb);      // the next head is on its way while this one is turned
+    float sq = 0.f;
+    if (m.on) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) sq += a[i] * a[i] + b[i] * b[i];
+    }
+    const float r = rsqrtf(group_sum<LG>(sq) * inv_d + p.eps);
+    const bool isq = h < p.q.heads;
+    if (m.on) {
+      float ya[P], yb[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float u = a[i] * r * (isq ? gqa[i] : gka[i]), v = b[i] * r * (isq ? gqb[i] : gkb[i]);
+        ya[i] = u * c[i] - v * s[i];
+        yb[i] = u * s[i] + v * c[i];
+      }
+      T* y = isq ? (T*)p.q.y + row * p.q.y_sr + (int64_t)h * p.q.y_sh : (T*)p.k.y + row * p.k.y_sr + (int64_t)(h - p.q.heads) * p.k.y_sh;
+      store_pairs<T, P, IL>(y, m, ya, yb);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) { a[i] = na[i]; b[i] = nb[i]; }
+  }
+}
+
+// gradient: blocks walk over tokens (grid-stride); one side (queries or keys) per blockIdx.y, so a lane sums one gamma gradient
+template <typename T, int P, int LG, bool IL>
+__global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(const MgldQkRope p, const int GT) {
+  extern __shared__ __attribute__((aligned(16))) float sg[];       // [groups][head_dim]
+  const MgldHeads& sd = blockIdx.y ? p.k : p.q;
+  const int grp = threadIdx.x / LG, slot = threadIdx.x % LG, d = p.head_dim;
+  constexpr int NG = 256 / LG;
+  const int TB = NG / GT;
+  const PairMap<P, IL> m(slot, d, p.rot_dim);
+  const float inv_d = 1.f / (float)d;
+  float ga[P], gb[P], da[P], db[P];
+  load_gamma<P, IL>(sd.gamma, m, ga, gb);
+#pragma unroll
+  for (int i = 0; i < P; ++i) { da[i] = 0.f; db[i] = 0.f; }
+  for (int64_t row = (int64_t)blockIdx.x * TB + grp / GT; row < p.rows; row += (int64_t)gridDim.x * TB) {
+    float c[P], s[P];
+    turn_of<P, IL>(p, row, m, c, s);
+    for (int h = grp % GT; h < sd.heads; h += GT) {
+      float a[P], b[P], ua[P], ub[P];
+      if (m.on) {
+        load_pairs<T, P, IL>((const T*)sd.x + row * sd.x_sr + (int64_t)h * sd.x_sh, m, a, b);
+        load_pairs<T, P, IL>((const T*)sd.dy + row * sd.dy_sr + (int64_t)h * sd.dy_sh, m, ua, ub);
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) { a[i] = 0.f; b[i] = 0.f; ua[i] = 0.f; ub[i] = 0.f; }
+      }
+      float sq = 0.f, dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float za = ua[i] * c[i] + ub[i] * s[i], zb = ub[i] * c[i] - ua[i] * s[i];
+        ua[i] = za;
+        ub[i] = zb;
+        sq += a[i] * a[i] + b[i] * b[i];
+        dot += za * ga[i] * a[i] + zb * gb[i] * b[i];
+      }
+      const float r = rsqrtf(group_sum<LG>(sq) * inv_d + p.eps);
+      dot = group_sum<LG>(dot) * r * inv_d;                          // mean_d(g z x r)
+      if (m.on) {
+        float ya[P], yb[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float xa = a[i] * r, xb = b[i] * r;
+          da[i] += ua[i] * xa;
+          db[i] += ub[i] * xb;
+          ya[i] = r * (ua[i] * ga[i] - xa * dot);
+          yb[i] = r * (ub[i] * gb[i] - xb * dot);
+        }
+        store_pairs<T, P, IL>((T*)sd.y + row * sd.y_sr + (int64_t)h * sd.y_sh, m, ya, yb);
+      }
+    }
+  }
+  if (!sd.dgamma) return;
+  if (m.on) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int ea = IL ? m.e0 + 2 * i : m.e0 + i, eb = IL ? m.e0 + 2 * i + 1 : m.e1 + i;
+      sg[grp * d + ea] = da[i];
+      sg[grp * d + eb] = db[i];
+    }
+  }
+  __syncthreads();
+  float* out = p.work + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * d;
+  for (int e = threadIdx.x; e < d; e += 256) {
+    float t = 0.f;
+    for (int g = 0; g < NG; ++g) t += sg[g * d + e];
+    out[e] = t;
+  }
+}
+
+// dgamma[e] = sum over the blocks' partial rows, fp64, fixed order: 16 columns x 16 segments of blocks per block
+__global__ __launch_bounds__(256) void qk_gamma_sum_kernel(const MgldQkRope p, const int nblk) {
+  __shared__ double sd[16][17];
+  float* out = blockIdx.y ? p.k.dgamma : p.q.dgamma;
+  if (!out) return;
+  const int col = threadIdx.x & 15, seg = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
+  double t = 0.;
+  if (e < p.head_dim)
+    for (int i = seg; i < nblk; i += 16) t += (double)p.work[((int64_t)blockIdx.y * nblk + i) * p.head_dim + e];
+  sd[seg][col] = t;
+  __syncthreads();
+  if (seg == 0 && e < p.head_dim) {
+    for (int i = 1; i < 16; ++i) t += sd[i][col];
+    out[e] = (float)t;
+  }
+}
+
+constexpr int QR_MAX_BLOCKS = 1024;
+
+// pairs a lane holds: 8 when sizes and addresses allow 16-byte vectors, else 4, else 0 (refused)
+int qr_pairs(const MgldQkRope* p, const bool grad) {
+  for (int P = 8; P >= 4; P /= 2) {
+    const int64_t bytes = 2 * P;
+    bool ok = p->head_dim % (2 * P) == 0 && p->rot_dim % (2 * P) == 0;
+    for (int i = 0; i < 2; ++i) {
+      const MgldHeads& h = i ? p->k : p->q;
+      if (!h.heads) continue;
+      ok = ok && ((uintptr_t)h.x | (uintptr_t)h.y) % bytes == 0 && h.x_sr % P == 0 && h.x_sh % P == 0 && h.y_sr % P == 0 && h.y_sh % P == 0;
+      if (grad) ok = ok && (uintptr_t)h.dy % bytes == 0 && h.dy_sr % P == 0 && h.dy_sh % P == 0;
+    }
+    if (ok) return P;
+  }
+  return 0;
+}
+
+int qr_check(const MgldQkRope* p, const bool grad) {
+  MGLD_REQUIRE(p && p->rows >= 0 && p->rows <= 0x7fffffff, "qk_norm_rope: rows");
+  MGLD_REQUIRE(p->head_dim >= 8 && p->head_dim <= 256 && p->head_dim % 8 == 0, "qk_norm_rope: head_dim must be a multiple of 8 up to 256");
+  MGLD_REQUIRE(p->rot_dim >= 0 && p->rot_dim <= p->head_dim && p->rot_dim % 8 == 0, "qk_norm_rope: rot_dim must be a multiple of 8 up to head_dim");
+  MGLD_REQUIRE(p->q.heads >= 0 && p->k.heads >= 0 && p->q.heads + p->k.heads > 0 && p->q.heads <= 65535 && p->k.heads <= 65535, "qk_norm_rope: heads");
+  MGLD_REQUIRE(p->eps >= 0.f, "qk_norm_rope: eps");
+  if (p->rows == 0) return MGLD_OK;
+  MGLD_REQUIRE(p->rot_dim == 0 || (p->pos && p->freqs), "qk_norm_rope: pos / freqs");
+  for (int i = 0; i < 2; ++i) {
+    const MgldHeads& h = i ? p->k : p->q;
+    MGLD_REQUIRE(!h.heads || (h.x && h.y && (!grad || h.dy)), "qk_norm_rope: null pointer");
+  }
+  MGLD_REQUIRE(qr_pairs(p, grad) > 0, "qk_norm_rope: pointers and strides must be multiples of 8 bytes");
+  return MGLD_OK;
+}
+
+int qr_grad_blocks(const int64_t rows, const int TB) {
+  const int64_t n = (rows + TB - 1) / TB;
+  return (int)(n < QR_MAX_BLOCKS ? n : QR_MAX_BLOCKS);
+}
+
+template <typename T, int P, int LG, bool IL>
+int qr_launch(const MgldQkRope& p, const bool grad, hipStream_t st) {
+  constexpr int NG = 256 / LG;
+  if (!grad) {
+    // many rows: a group walks several heads of its token (sines once per token); few rows: one head per group, heads over blockIdx.y
+    const int H = p.q.heads + p.k.heads;
+    int GT = NG;
+    if (p.rows >= 4096) while (GT > 1 && GT * 4 > H) GT /= 2;
+    else while (GT > 1 && GT / 2 >= H) GT /= 2;
+    const int gy = p.rows >= 4096 ? 1 : cdiv(H, GT);
+    const int TB = NG / GT;
+    qk_norm_rope_kernel<T, P, LG, IL><<<dim3(cdiv(p.rows, TB), gy), 256, 0, st>>>(p, GT);
+    return mgld_check_launch("qk_norm_rope");
+  }
+  const int hmax = p.q.heads > p.k.heads ? p.q.heads : p.k.heads;
+  int GT = NG;
+  while (GT > 1 && GT > hmax) GT /= 2;
+  const int nb = qr_grad_blocks(p.rows, NG / GT);
+  const bool gam = p.q.dgamma || p.k.dgamma;
+  qk_norm_rope_grad_kernel<T, P, LG, IL><<<dim3(nb, 2), 256, NG * p.head_dim * 4, st>>>(p, GT);
+  if (gam) qk_gamma_sum_kernel<<<dim3(cdiv(p.head_dim, 16), 2), 256, 0, st>>>(p, nb);
+  return mgld_check_launch("qk_norm_rope_grad");
+}
+
+template <typename T, int P, bool IL>
+int qr_lanes(const MgldQkRope& p, const bool grad, hipStream_t st) {
+  const int lanes = cdiv(p.head_dim, 2 * P);
+  if (lanes <= 4) return qr_launch<T, P, 4, IL>(p, grad, st);
+  if (lanes <= 8) return qr_launch<T, P, 8, IL>(p, grad, st);
+  if (lanes <= 16) return qr_launch<T, P, 16, IL>(p, grad, st);
+  return qr_launch<T, P, 32, IL>(p, grad, st);
+}
+template <typename T, int P>
+int qr_layout(const MgldQkRope& p, const bool grad, hipStream_t st) {
+  return p.interleaved ? qr_lanes<T, P, true>(p, grad, st) : qr_lanes<T, P, false>(p, grad, st);
+}
+int qr_run(const MgldQkRope& p, const bool grad, hipStream_t st) {
+  const bool wide = qr_pairs(&p, grad) == 8;
+  if (p.bf16) return wide ? qr_layout<bf16, 8>(p, grad, st) : qr_layout<bf16, 4>(p, grad, st);
+  return wide ? qr_layout<f16, 8>(p, grad, st) : qr_layout<f16, 4>(p, grad, st);
+}
+
+}  // namespace
+
+extern "C" int mgld_qk_norm_rope(const MgldQkRope* p, void* stream) {
+  const int rc = qr_check(p, false);
+  if (rc || p->rows == 0) return rc;
+  return qr_run(*p, false, (hipStream_t)stream);
+}
+
+extern "C" int64_t mgld_qk_norm_rope_grad_work(const MgldQkRope* p) {
+  if (!p || p->rows <= 0) return 0;
+  return (int64_t)2 * (p->rows < QR_MAX_BLOCKS ? p->rows : QR_MAX_BLOCKS) * p->head_dim * 4;
+}
+
+extern "C" int mgld_qk_norm_rope_grad(const MgldQkRope* p, void* stream) {
+  const int rc = qr_check(p, true);
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (p->rows == 0) {          // no rows: the sums over them are zero
+    if (p->q.dgamma || p->k.dgamma) qk_gamma_sum_kernel<<<dim3(cdiv(p->head_dim, 16), 2), 256, 0, st>>>(*p, 0);
+    return mgld_check_launch("qk_norm_rope_grad");
+  }
+  if (p->q.dgamma || p->k.dgamma)
+    MGLD_REQUIRE(p->work && p->work_bytes >= mgld_qk_norm_rope_grad_work(p) && (uintptr_t)p->work % 16 == 0, "qk_norm_rope_grad: work buffer too small");
+  return qr_run(*p, true, st);
+}

@@ -51,6 +51,29 @@ class MgldAttn(C.Structure):
     ]
 
 
+class MgldHeads(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("dy", C.c_void_p), ("gamma", C.c_void_p), ("dgamma", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("x_sr", "x_sh", "y_sr", "y_sh", "dy_sr", "dy_sh", "heads")]
+
+
+class MgldQkRope(C.Structure):
+    _fields_ = [("q", MgldHeads), ("k", MgldHeads), ("pos", C.c_void_p), ("freqs", C.c_void_p), ("work", C.c_void_p),
+                ("work_bytes", C.c_int64), ("rows", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("pos64", "head_dim", "rot_dim", "interleaved", "bf16")] + [("eps", C.c_float)]
+
+
+class MgldMaskAttn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("Q", "K", "V", "O", "lse")] + \
+               [(n + s, C.c_int64) for n in ("q", "k", "v", "o") for s in ("_sb", "_si", "_sh")] + \
+               [(n, C.c_void_p) for n in ("slopes", "rel", "doc_q", "doc_k", "prefix", "kv_len")] + \
+               [("doc_q_sb", C.c_int64), ("doc_k_sb", C.c_int64)] + \
+               [(n, C.c_void_p) for n in ("dO", "dQ", "dK", "dV", "dRel")] + \
+               [(n + s, C.c_int64) for n in ("do", "dq", "dk", "dv") for s in ("_sb", "_si", "_sh")] + \
+               [("work", C.c_void_p), ("work_bytes", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("batch", "heads", "kv_heads", "Nq", "Nkv", "head_dim", "reach", "q_pos0", "q_from_end", "causal", "bf16")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
 # every symbol include/mgld_hip.h declares (tests check the library exports all of them)
 EXPORTS = [
     "mgld_version", "mgld_last_error", "mgld_device_info",
@@ -69,6 +92,9 @@ EXPORTS = [
     "mgld_resize_bicubic", "mgld_resize_bilinear_crop", "mgld_reflect_pad", "mgld_replicate_pad", "mgld_to_uint8_hwc",
     "mgld_hp_chunks", "mgld_hp_gn_stats", "mgld_hp_gn_split", "mgld_hp_softmax_rows",
     "mgld_conv_f32", "mgld_instnorm_chunks", "mgld_instnorm_f32", "mgld_nchw_to_nhwc_f32",
+    "mgld_qk_norm_rope", "mgld_qk_norm_rope_grad_work", "mgld_qk_norm_rope_grad",
+    "mgld_masked_attention_work", "mgld_masked_attention", "mgld_masked_attention_grad_work", "mgld_masked_attention_grad",
+    "mgld_rel_bias", "mgld_rel_bias_grad",
     "mgld_avgpool2", "mgld_corr_lookup", "mgld_gru_rh", "mgld_gru_gate", "mgld_flow_update", "mgld_convex_upsample",
 ]
 
@@ -89,6 +115,8 @@ def lib():
         _lib = C.CDLL(os.environ.get("MGLD_HIP_LIB") or _LIB_PATH)
         _lib.mgld_last_error.restype = C.c_char_p
         _lib.mgld_gn_chunks.restype = C.c_int
+        for f in ("mgld_qk_norm_rope_grad_work", "mgld_masked_attention_work", "mgld_masked_attention_grad_work"):
+            getattr(_lib, f).restype = C.c_int64
     return _lib
 
 
@@ -912,3 +940,439 @@ def hp_softmax_rows(S):
     _f32(S)
     _chk(lib().mgld_hp_softmax_rows(_p(S), C.c_int64(S.shape[0]), S.shape[1], _ld(S), stream_ptr()), "hp_softmax_rows")
     return S
+
+
+# ---- transformer operators: norms of the query / key heads with the rotation, masked attention, relative bias -------------------------------
+# Tensors are fp16 or bf16 (statistics, biases and their gradients fp32), with any batch / row / head strides and unit stride along the head
+# dimension.  There is no autograd: the gradient is its own call.  Results the caller does not pass are allocated; while a graph is being
+# captured they and `work` have to be passed (memory handed back to torch's allocator would be reused under the graph).  Two calls whose work
+# may overlap in time (two streams, two captured graphs) need work buffers of their own.
+class _OnDevice:
+    """makes the tensors' device the current one for a call (the launch goes to its current stream)"""
+
+    def __init__(self, t):
+        self.dev = t.device
+
+    def __enter__(self):
+        self.ctx = None
+        if self.dev.index is not None and self.dev.index != torch.cuda.current_device():
+            self.ctx = torch.cuda.device(self.dev)
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        return False
+
+
+def _same_device(what, *ts):
+    _req_cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if not (len(devs) <= 1):
+        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devs))}")
+
+
+class _Memory:
+    """the memory of a tensor as numpy's overlap solver sees it (never read)"""
+
+    def __init__(self, t):
+        es = t.element_size()
+        self.__array_interface__ = {"version": 3, "shape": tuple(t.shape), "strides": tuple(st * es for st in t.stride()),
+                                    "typestr": f"|V{es}", "data": (t.data_ptr(), True)}
+
+
+def _overlap(a, b):
+    """do two tensors share memory?  Exact for strided views (column blocks of one buffer do not); True where that is too hard to tell"""
+    if a is None or b is None or a.numel() == 0 or b.numel() == 0:
+        return False
+    ends = [t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
+    if ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr():
+        return False
+    import numpy as np
+    try:
+        return bool(np.shares_memory(np.asarray(_Memory(a)), np.asarray(_Memory(b)), max_work=100000))
+    except Exception:
+        return True
+
+
+def _same_view(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and _strides(a) == _strides(b)
+
+
+def _strides(t):
+    """strides but the last one's; a dimension of one element has none"""
+    return tuple(0 if n == 1 else st for n, st in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def _heads_view(what, name, t, dim, dtype=None, shape=None):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: {name} must be a tensor")
+    if not (t.dtype in (torch.float16, torch.bfloat16)):
+        raise ValueError(f"{what}: {name} must be float16 or bfloat16, got {t.dtype}")
+    if not (dtype is None or t.dtype == dtype):
+        raise ValueError(f"{what}: {name} is {t.dtype}, the call is {dtype}")
+    if not (t.dim() == dim and (t.shape[-1] <= 1 or t.stride(-1) == 1)):
+        raise ValueError(f"{what}: {name} must have {dim} dimensions and unit stride along the last, got {tuple(t.shape)} {t.stride()}")
+    if not (shape is None or tuple(t.shape) == tuple(shape)):
+        raise ValueError(f"{what}: {name} must be {shape}, got {tuple(t.shape)}")
+
+
+def _out(what, name, t, like, capturing, inputs=(), inplace=(), shape=None, dtype=None):
+    """an output the caller passed (checked) or a new one"""
+    shape, dtype = tuple(like.shape if shape is None else shape), like.dtype if dtype is None else dtype
+    if t is None:
+        if capturing:
+            raise ValueError(f"{what}: pass {name}= while a graph is being captured")
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if not (tuple(t.shape) == shape and t.dtype == dtype and t.device == like.device):
+        raise ValueError(f"{what}: {name} must be {dtype} {shape} on {like.device}")
+    if not (t.numel() == 0 or all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride()))):
+        raise ValueError(f"{what}: {name} must not repeat its elements")
+    for x in inputs:
+        if x is not None and not any(x is y and _same_view(t, y) for y in inplace):
+            if _overlap(t, x):
+                raise ValueError(f"{what}: {name} overlaps another tensor of the call")
+    return t
+
+
+def _vec(what, name, t, n, dtype, like):
+    if t is not None:
+        if not (isinstance(t, torch.Tensor) and t.dtype == dtype and tuple(t.shape) == n and t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous {dtype} {n}")
+        if not (t.device == like.device):
+            raise ValueError(f"{what}: {name} must be on {like.device}")
+    return t
+
+
+def _work(what, work, nbytes, like, capturing, others=()):
+    if nbytes == 0:
+        return None
+    if work is None:
+        if capturing:
+            raise ValueError(f"{what}: pass work= ({nbytes} bytes) while a graph is being captured")
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    if not (work.is_contiguous() and work.device == like.device and work.numel() * work.element_size() >= nbytes and work.data_ptr() % 16 == 0):
+        raise ValueError(f"{what}: work must be a contiguous, 16-byte aligned device buffer of at least {nbytes} bytes")
+    for t in others:
+        if _overlap(work, t):
+            raise ValueError(f"{what}: work overlaps another tensor of the call")
+    return work
+
+
+def _set_work(p, work):
+    if work is not None:
+        p.work, p.work_bytes = work.data_ptr(), work.numel() * work.element_size()
+
+
+def _capturing():
+    return torch.cuda.is_current_stream_capturing()
+
+
+def rope_freqs(rot_dim, base=10000.0, device="cuda"):
+    """float64 [rot_dim / 2]: radians per position of the rotation's pairs, base^(-2 j / rot_dim)"""
+    return base ** (-2.0 * torch.arange(rot_dim // 2, dtype=torch.float64, device=device) / max(1, rot_dim))
+
+
+def _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps, interleaved):
+    for n, t in (("q", q), ("k", k)):
+        if t is not None:
+            _heads_view(what, n, t, 3)
+    x = q if q is not None else k
+    if not (x is not None):
+        raise ValueError(f"{what}: q or k")
+    rows, d = x.shape[0], x.shape[2]
+    for n, t in (("q", q), ("k", k)):
+        if t is not None:
+            if not (t.dtype == x.dtype and t.shape[0] == rows and t.shape[2] == d):
+                raise ValueError(f"{what}: q and k must agree in type, rows and head size")
+    _same_device(what, q, k, pos, freqs, q_gamma, k_gamma)
+    if not (d % 8 == 0 and 8 <= d <= 256):
+        raise ValueError(f"{what}: head size {d}: a multiple of 8 up to 256")
+    rot = 0
+    if freqs is not None:
+        if not (freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous()):
+            raise ValueError(f"{what}: freqs must be contiguous float64 [rot_dim / 2]")
+        rot = 2 * freqs.shape[0]
+        if not (rot <= d and rot % 8 == 0):
+            raise ValueError(f"{what}: rot_dim {rot}: a multiple of 8 up to the head size")
+    if rot:
+        if not (pos is not None and pos.dtype in (torch.int32, torch.int64) and tuple(pos.shape) == (rows,) and pos.is_contiguous()):
+            raise ValueError(f"{what}: pos must be contiguous int32 or int64 [{rows}]")
+    _vec(what, "q_gamma", q_gamma, (d,), torch.float32, x)
+    _vec(what, "k_gamma", k_gamma, (d,), torch.float32, x)
+    if not (eps >= 0):
+        raise ValueError(f"{what}: eps must not be negative")
+    p = MgldQkRope()
+    p.rows, p.head_dim, p.rot_dim, p.interleaved, p.bf16, p.eps = rows, d, rot, int(bool(interleaved)), int(x.dtype == torch.bfloat16), eps
+    if rot:
+        p.pos, p.freqs, p.pos64 = pos.data_ptr(), freqs.data_ptr(), int(pos.dtype == torch.int64)
+    return p, x
+
+
+def _side(h, x, y, dy=None, gamma=None, dgamma=None):
+    h.heads = x.shape[1]
+    h.x, (h.x_sr, h.x_sh) = x.data_ptr(), _strides(x)
+    h.y, (h.y_sr, h.y_sh) = y.data_ptr(), _strides(y)
+    if dy is not None:
+        h.dy, (h.dy_sr, h.dy_sh) = dy.data_ptr(), _strides(dy)
+    h.gamma, h.dgamma = _p(gamma).value, _p(dgamma).value
+
+
+def qk_norm_rope(q, k, pos, freqs, *, q_gamma=None, k_gamma=None, eps=1e-6, interleaved=False, q_out=None, k_out=None):
+    """Root-mean-square norm of every query and key head and the rotation of its first 2 * len(freqs) elements, one pass (include/mgld_hip.h).
+    q [rows, heads, d], k [rows, kv_heads, d] (either may be None); pos int32 / int64 [rows]; freqs float64 (rope_freqs; None: no rotation);
+    gammas fp32 [d].  q_out / k_out may be q / k themselves.  -> (q_out, k_out)"""
+    what = "qk_norm_rope"
+    p, x = _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps, interleaved)
+    with _OnDevice(x):
+        cap = _capturing()
+        ins = (q, k, pos, freqs, q_gamma, k_gamma)
+        if q is not None:
+            q_out = _out(what, "q_out", q_out, q, cap, ins, (q,))
+            _heads_view(what, "q_out", q_out, 3)
+            _side(p.q, q, q_out, gamma=q_gamma)
+        if k is not None:
+            k_out = _out(what, "k_out", k_out, k, cap, ins + (q_out,), (k,))
+            _heads_view(what, "k_out", k_out, 3)
+            _side(p.k, k, k_out, gamma=k_gamma)
+        _chk(lib().mgld_qk_norm_rope(C.byref(p), stream_ptr()), what)
+    return (q_out if q is not None else None), (k_out if k is not None else None)
+
+
+def qk_norm_rope_grad_work_bytes(rows, head_dim):
+    p = MgldQkRope()
+    p.rows, p.head_dim = rows, head_dim
+    return int(lib().mgld_qk_norm_rope_grad_work(C.byref(p)))
+
+
+def qk_norm_rope_grad(q, k, pos, freqs, dq_out, dk_out, *, q_gamma=None, k_gamma=None, eps=1e-6, interleaved=False, dq=None, dk=None,
+                      dq_gamma=None, dk_gamma=None, work=None):
+    """Gradient of qk_norm_rope: q, k are ITS inputs, dq_out / dk_out the gradients of its results.  -> (dq, dk, dq_gamma, dk_gamma); a gamma's
+    gradient is fp32 [d], None where that gamma is.  dq may be dq_out or q (dk likewise)."""
+    what = "qk_norm_rope_grad"
+    p, x = _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps, interleaved)
+    if not ((q is None) == (dq_out is None) and (k is None) == (dk_out is None)):
+        raise ValueError(f"{what}: a gradient for each of q, k")
+    _same_device(what, x, dq_out, dk_out)
+    with _OnDevice(x):
+        cap = _capturing()
+        ins = (q, k, pos, freqs, q_gamma, k_gamma, dq_out, dk_out)
+        outs = []
+        for n, t, g, gamma, dt, dg, side in (("q", q, dq_out, q_gamma, dq, dq_gamma, p.q), ("k", k, dk_out, k_gamma, dk, dk_gamma, p.k)):
+            if t is None:
+                outs += [None, None]
+                continue
+            _heads_view(what, f"d{n}_out", g, 3, x.dtype, t.shape)
+            dt = _out(what, "d" + n, dt, t, cap, ins + tuple(outs), (t, g))
+            _heads_view(what, "d" + n, dt, 3)
+            outs.append(dt)
+            if gamma is not None:
+                dg = _out(what, f"d{n}_gamma", dg, gamma, cap, ins + tuple(outs))
+                if not dg.is_contiguous():
+                    raise ValueError(f"{what}: d{n}_gamma must be contiguous")
+            else:
+                dg = None
+            outs.append(dg)
+            _side(side, t, dt, g, gamma, dg)
+        if outs[1] is not None or outs[3] is not None:
+            work = _work(what, work, int(lib().mgld_qk_norm_rope_grad_work(C.byref(p))), x, cap, ins + tuple(outs))
+            _set_work(p, work)
+        _chk(lib().mgld_qk_norm_rope_grad(C.byref(p), stream_ptr()), what)
+    return outs[0], outs[2], outs[1], outs[3]
+
+
+def _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0):
+    """the checked problem without outputs"""
+    _heads_view(what, "q", q, 4)
+    _heads_view(what, "k", k, 4, q.dtype)
+    _heads_view(what, "v", v, 4, q.dtype, k.shape)
+    B, Nq, H, d = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    if not (k.shape[0] == B and k.shape[3] == d):
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch and head size")
+    if not (Hk > 0 and H > 0 and H % Hk == 0):
+        raise ValueError(f"{what}: {H} query heads over {Hk} key heads")
+    if not (d % 8 == 0 and 8 <= d <= 128):
+        raise ValueError(f"{what}: head size {d}: a multiple of 8 up to 128")
+    _same_device(what, q, k, v, slopes, rel, prefix, kv_len)
+    scale = float(d) ** -0.5 if scale is None else float(scale)
+    softcap = float(softcap or 0.0)
+    if not (0.0 < scale < 3e38 and 0.0 <= softcap < 3e38):
+        raise ValueError(f"{what}: scale must be positive, softcap not negative")
+    if not (slopes is None or rel is None):
+        raise ValueError(f"{what}: slopes or rel, not both")
+    p = MgldMaskAttn()
+    p.batch, p.heads, p.kv_heads, p.Nq, p.Nkv, p.head_dim = B, H, Hk, Nq, Nk, d
+    p.bf16, p.causal, p.scale, p.softcap = int(q.dtype == torch.bfloat16), int(bool(causal)), scale, softcap
+    p.slopes = _p(_vec(what, "slopes", slopes, (H,), torch.float32, q)).value
+    if rel is not None:
+        if not (rel.dim() == 2 and rel.shape[1] % 2 == 1 and rel.shape[1] <= 2049):
+            raise ValueError(f"{what}: rel must be [heads, 2 * reach + 1] with reach up to 1024")
+        _vec(what, "rel", rel, (H, rel.shape[1]), torch.float32, q)
+        p.rel, p.reach = rel.data_ptr(), rel.shape[1] // 2
+    if docs is not None:
+        if isinstance(docs, torch.Tensor):
+            if not (Nq == Nk):
+                raise ValueError(f"{what}: one docs tensor needs as many queries as keys; pass (doc_q, doc_k)")
+            docs = (docs, docs)
+        for n, t, m in (("doc_q", docs[0], Nq), ("doc_k", docs[1], Nk)):
+            if not (t.dtype == torch.int32 and tuple(t.shape) == (B, m) and (m <= 1 or t.stride(1) == 1)):
+                raise ValueError(f"{what}: {n} must be int32 [{B}, {m}] with unit stride")
+        _same_device(what, q, *docs)
+        p.doc_q, p.doc_k = docs[0].data_ptr() or None, docs[1].data_ptr() or None
+        p.doc_q_sb, p.doc_k_sb = _strides(docs[0])[0], _strides(docs[1])[0]
+    if not (prefix is None or causal):
+        raise ValueError(f"{what}: prefix needs causal=True")
+    p.prefix = _p(_vec(what, "prefix", prefix, (B,), torch.int32, q)).value
+    p.kv_len = _p(_vec(what, "kv_len", kv_len, (B,), torch.int32, q)).value
+    if q_pos0 is None:
+        p.q_from_end = 1
+    else:
+        if not (abs(int(q_pos0)) <= 1 << 30):
+            raise ValueError(f"{what}: q_pos0")
+        p.q_pos0 = int(q_pos0)
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _put(p, n, n.upper(), t)
+    ins = (q, k, v, slopes, rel, prefix, kv_len) + (tuple(docs) if docs is not None else ())
+    return p, ins
+
+
+def _put(p, n, field, t):
+    setattr(p, field, t.data_ptr())
+    for a, st in zip(("_sb", "_si", "_sh"), _strides(t)):
+        setattr(p, n + a, st)
+
+
+def masked_attention(q, k, v, *, scale=None, causal=False, softcap=0.0, slopes=None, rel=None, docs=None, prefix=None, kv_len=None, q_pos0=None,
+                     o=None, lse=None, work=None):
+    """softmax(scores) v with capped scores, a distance bias and masks (include/mgld_hip.h has the formula).
+    q [B, Nq, heads, d], k / v [B, Nkv, kv_heads, d] (heads a multiple of kv_heads, d a multiple of 8 up to 128).
+    scale: default d^-1/2.  softcap: scores become softcap * tanh(score / softcap).
+    slopes: fp32 [heads], bias -slope * |distance|; or rel: fp32 [heads, 2 * reach + 1], bias by clamped distance (rel_bias).
+    causal; prefix: int32 [B], keys below it are seen by every query (with causal).  docs: int32 document numbers [B, N], or (doc_q, doc_k):
+    a query sees keys of its own document, negative = padding.  kv_len: int32 [B], keys at or past it are never seen (nor read).
+    q_pos0: position of the first query; None: the queries are the last ones before kv_len (of a cache's newest tokens).
+    A query that sees nothing gives 0 (lse -inf).  -> (o like q, lse fp32 [B, heads, Nq])"""
+    what = "masked_attention"
+    p, ins = _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
+    B, Nq, H, d = q.shape
+    with _OnDevice(q):
+        cap = _capturing()
+        o = _out(what, "o", o, q, cap, ins)
+        _heads_view(what, "o", o, 4)
+        _put(p, "o", "O", o)
+        lse = _out(what, "lse", lse, q, cap, ins + (o,), shape=(B, H, Nq), dtype=torch.float32)
+        if not lse.is_contiguous():
+            raise ValueError(f"{what}: lse must be contiguous")
+        p.lse = lse.data_ptr()
+        work = _work(what, work, int(lib().mgld_masked_attention_work(C.byref(p))), q, cap, ins + (o, lse))
+        _set_work(p, work)
+        _chk(lib().mgld_masked_attention(C.byref(p), stream_ptr()), what)
+    return o, lse
+
+
+def masked_attention_grad(q, k, v, o, lse, do, *, scale=None, causal=False, softcap=0.0, slopes=None, rel=None, docs=None, prefix=None, kv_len=None,
+                          q_pos0=None, dq=None, dk=None, dv=None, drel=None, work=None):
+    """Gradient of masked_attention, called with the same options, its results o and lse, and do = the gradient of o.
+    -> (dq, dk, dv, drel): dk / dv summed over the query heads that share them, zeros where no query sees the key; drel fp32 like rel (None
+    without rel).  Sums have a fixed order: equal calls give equal bits."""
+    what = "masked_attention_grad"
+    p, ins = _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
+    B, Nq, H, d = q.shape
+    _heads_view(what, "o", o, 4, q.dtype, q.shape)
+    _heads_view(what, "do", do, 4, q.dtype, q.shape)
+    _same_device(what, q, o, lse, do)
+    _vec(what, "lse", lse, (B, H, Nq), torch.float32, q)
+    ins = ins + (o, lse, do)
+    with _OnDevice(q):
+        cap = _capturing()
+        _put(p, "o", "O", o)
+        _put(p, "do", "dO", do)
+        p.lse = lse.data_ptr()
+        outs = []
+        for n, t, like in (("q", dq, q), ("k", dk, k), ("v", dv, v)):
+            t = _out(what, "d" + n, t, like, cap, ins + tuple(outs))
+            _heads_view(what, "d" + n, t, 4)
+            _put(p, "d" + n, "d" + n.upper(), t)
+            outs.append(t)
+        if rel is not None:
+            drel = _out(what, "drel", drel, rel, cap, ins + tuple(outs))
+            if not drel.is_contiguous():
+                raise ValueError(f"{what}: drel must be contiguous")
+            p.dRel = drel.data_ptr()
+            outs.append(drel)
+        else:
+            outs.append(None)
+        work = _work(what, work, int(lib().mgld_masked_attention_grad_work(C.byref(p))), q, cap, ins + tuple(outs))
+        _set_work(p, work)
+        _chk(lib().mgld_masked_attention_grad(C.byref(p), stream_ptr()), what)
+    return tuple(outs)
+
+
+class RelBuckets:
+    """Which bucket each distance -reach .. reach (key - query) belongs to: `index` int32 [2 * reach + 1] on the device."""
+
+    def __init__(self, num_buckets, max_distance, bidirectional, device):
+        self.num_buckets, self.max_distance, self.bidirectional, self.reach = num_buckets, max_distance, bidirectional, max_distance
+        self.index = torch.tensor([rel_bucket(i, num_buckets, max_distance, bidirectional) for i in range(-max_distance, max_distance + 1)],
+                                  dtype=torch.int32, device=device)
+
+
+def rel_bucket(distance, num_buckets, max_distance, bidirectional=True):
+    """bucket of a distance (key - query): half of the buckets for keys ahead when bidirectional (keys ahead count as 0 otherwise); of nb
+    buckets the first nb / 2 hold one distance each, the others grow logarithmically up to max_distance.  By whole numbers: distance n is at or past
+    the border of bucket exact + j where (n / exact)^(nb - exact) >= (max_distance / exact)^j."""
+    nb, first = num_buckets, 0
+    if bidirectional:
+        nb //= 2
+        first = nb if distance > 0 else 0
+        n = abs(distance)
+    else:
+        n = max(-distance, 0)
+    exact = nb // 2
+    if n < exact:
+        return first + n
+    m, j = nb - exact, 0
+    while j + 1 < m and n ** m * exact ** (j + 1) >= max_distance ** (j + 1) * exact ** m:
+        j += 1
+    return first + exact + j
+
+
+def rel_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
+    """the plan rel_bias and rel_bias_grad take (made once, like the table); max_distance <= 1024"""
+    nb = num_buckets // 2 if bidirectional else num_buckets
+    if not ((not bidirectional or num_buckets % 2 == 0) and nb >= 2):
+        raise ValueError("rel_buckets: at least two buckets a side")
+    if not (nb // 2 < max_distance <= 1024):
+        raise ValueError("rel_buckets: max_distance must exceed the buckets of one distance each and stay within 1024")
+    return RelBuckets(num_buckets, max_distance, bool(bidirectional), device)
+
+
+def rel_bias(table, plan, out=None):
+    """learned bias table fp32 [buckets, heads] -> fp32 [heads, 2 * reach + 1], the `rel` of masked_attention"""
+    what = "rel_bias"
+    _same_device(what, table, plan.index)
+    if not (table.dim() == 2):
+        raise ValueError(f"{what}: table must be [buckets, heads]")
+    _vec(what, "table", table, (plan.num_buckets, table.shape[1]), torch.float32, table)
+    with _OnDevice(table):
+        out = _out(what, "out", out, table, _capturing(), (table, plan.index), shape=(table.shape[1], 2 * plan.reach + 1))
+        if not out.is_contiguous():
+            raise ValueError(f"{what}: out must be contiguous")
+        _chk(lib().mgld_rel_bias(_p(table), _p(plan.index), _p(out), plan.num_buckets, table.shape[1], 2 * plan.reach + 1, stream_ptr()), what)
+    return out
+
+
+def rel_bias_grad(drel, plan, out=None):
+    """gradient of rel_bias: drel fp32 [heads, 2 * reach + 1] -> the table's, fp32 [buckets, heads]"""
+    what = "rel_bias_grad"
+    _same_device(what, drel, plan.index)
+    if not (drel.dim() == 2):
+        raise ValueError(f"{what}: drel must be [heads, 2 * reach + 1]")
+    _vec(what, "drel", drel, (drel.shape[0], 2 * plan.reach + 1), torch.float32, drel)
+    with _OnDevice(drel):
+        out = _out(what, "out", out, drel, _capturing(), (drel, plan.index), shape=(plan.num_buckets, drel.shape[0]))
+        if not out.is_contiguous():
+            raise ValueError(f"{what}: out must be contiguous")
+        _chk(lib().mgld_rel_bias_grad(_p(drel), _p(plan.index), _p(out), plan.num_buckets, drel.shape[0], 2 * plan.reach + 1, stream_ptr()), what)
+    return out

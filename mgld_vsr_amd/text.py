@@ -14,6 +14,7 @@ outside the per-step hot path.  Two modes:
   data file (found in an installed open_clip / clip package or via $MGLD_BPE_VOCAB).  The empty prompt — the only one the
   inference scripts use — tokenises to [SOT, EOT, 0, ...] without the table.
 """
+import os
 import warnings
 
 import torch
@@ -155,13 +156,20 @@ class FrozenOpenCLIPEmbedder(nn.Module):
         x0 = (m.token_embedding.weight.detach()[tokens] + m.positional_embedding.detach()).float()      # host gather
         x = x0.reshape(n * L, W).to(eng.device, torch.float16).contiguous()
         blocks = m.transformer.resblocks
+        # MGLD_TEXT_ATTN=1: the causal attention as one fused launch (same arithmetic, other roundings); default: the recorded four-launch form
+        fused = os.environ.get("MGLD_TEXT_ATTN", "0") == "1" and d % 8 == 0 and d <= 128
+        lse = eng.arena.alloc((n, H, L), torch.float32) if fused else None
         for blk in list(blocks)[:len(blocks) - self.layer_idx]:
             a = blk.attn
             h = eng.layernorm(x, eng.f32("g", blk.ln_1.weight), eng.f32("b", blk.ln_1.bias), blk.ln_1.eps)
             qkv = eng.linear(h, eng.weight("w", (a.in_proj_weight,), lambda w: w), eng.f32("b", a.in_proj_bias))   # [nL, 3W]
-            # per (sequence, head): S = q k^T / sqrt(d) (fp32), causal softmax, O = P V with V^T from a batched NT GEMM
             o = eng.arena.alloc((n * L, W), torch.float16)
-            for b in range(n):
+            if fused:                        # all sequences and heads in one launch, no scores in memory
+                q, k, v = (qkv[:, i * W:(i + 1) * W].view(n, L, H, d) for i in range(3))
+                hip.masked_attention(q, k, v, causal=True, o=o.view(n, L, H, d), lse=lse)
+                eng.launches += 1
+            # per (sequence, head): S = q k^T / sqrt(d) (fp32), causal softmax, O = P V with V^T from a batched NT GEMM
+            for b in range(0 if fused else n):
                 r = slice(b * L, (b + 1) * L)
                 S = eng.arena.alloc((H * L, L), torch.float32)
                 hip.igemm(qkv[r, 0:W], qkv[r, W:2 * W], S, M=L, N=L, K=d, alpha=float(d) ** -0.5, batch=H, strideA=d, strideW=d,
