@@ -521,7 +521,7 @@ int64_t mgld_masked_attention_work(const MgldMaskAttn* p);
 int mgld_masked_attention(const MgldMaskAttn* p, void* stream);
 /* From the forward's o and lse: dV = P^T dO, dS = P (dO V^T - rowsum(dO o)), dRel = dS summed over rows, batch and equal distances,
  * dQ = scale dT K, dK = scale dT^T Q with dT = dS (1 - (u / softcap)^2); K / V gradients summed over the query heads that share them.
- * Every sum has a fixed order.  Rows of dK / dV that no query sees are written as zeros. */
+ * (rowsum(dO o) is summed from P and dP in fp32: O is not read.)  Every sum has a fixed order.  Rows of dK / dV that no query sees are written as zeros. */
 int64_t mgld_masked_attention_grad_work(const MgldMaskAttn* p);
 int mgld_masked_attention_grad(const MgldMaskAttn* p, void* stream);
 

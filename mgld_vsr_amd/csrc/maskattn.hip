@@ -537,7 +537,7 @@ int ma_check(const MgldMaskAttn* p, const bool grad) {
   MGLD_REQUIRE((p->doc_q != nullptr) == (p->doc_k != nullptr) || p->Nq == 0 || p->Nkv == 0, "masked_attention: doc_q and doc_k go together");
   if (p->batch == 0 || (p->Nq == 0 && !grad)) return MGLD_OK;
   if (p->Nq > 0) {
-    MGLD_REQUIRE(ma_aligned(p->Q, p->q_sb, p->q_si, p->q_sh) && ma_aligned(p->O, p->o_sb, p->o_si, p->o_sh), "masked_attention: q / o must be 16-byte aligned with strides of multiples of 8");
+    MGLD_REQUIRE(ma_aligned(p->Q, p->q_sb, p->q_si, p->q_sh) && (grad || ma_aligned(p->O, p->o_sb, p->o_si, p->o_sh)), "masked_attention: q / o must be 16-byte aligned with strides of multiples of 8");
     if (grad) MGLD_REQUIRE(ma_aligned(p->dO, p->do_sb, p->do_si, p->do_sh) && ma_aligned(p->dQ, p->dq_sb, p->dq_si, p->dq_sh) && p->lse, "masked_attention_grad: do / dq alignment, lse");
   }
   // a tile's rows are addressed with 31-bit byte offsets (its base with 64 bits)

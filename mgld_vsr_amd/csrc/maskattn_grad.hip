@@ -1,12 +1,13 @@
 // maskattn_grad.hip — gradient of the masked attention (maskattn.hip) from its output and log-sum-exp.
 //
-//   P = exp(s - lse),  dP = dO V^T,  D_i = dO_i . o_i,  dS = P (dP - D),  dT = dS (1 - (u / softcap)^2)
+//   P = exp(s - lse),  dP = dO V^T,  D = rowsum(P dP) = dO . o,  dS = P (dP - D),  dT = dS (1 - (u / softcap)^2)
 //   dV = P^T dO,  dQ = scale dT K,  dK = scale dT^T Q,  dRel[h][c] = sum of dS over the pairs at distance c
 //
-// Two passes over the visible pairs, each recomputing the scores, so that every sum has one owner and a fixed order (no atomics; 7 products
+// Passes over the visible pairs that recompute the scores, so that every sum has one owner and a fixed order (no atomics; 9 products
 // instead of 5):
-//  * ma_dq_kernel, per 128 query rows: S^T = K Q^T and dP^T = V dO^T (a lane holds keys of ONE query row), dQ^T += K^T dT^T; K read both ways
-//    from one LDS tile.  With a relative bias it also adds dS along the diagonals: a 32 x 32 block goes through LDS, lane c sums diagonal c;
+//  * ma_dq_kernel, per 128 query rows, goes over the keys twice: D = sum P dP first (from the rounded o, D would be off by 2^-9 sum |do o| in bf16, which
+//    the sums over rows keep: dRel lost three digits), then S^T = K Q^T and dP^T = V dO^T again (a lane holds keys of ONE query row) and
+//    dQ^T += K^T dT^T; K read both ways from one LDS tile.  With a relative bias it also adds dS along the diagonals: a 32 x 32 block goes through LDS, lane c sums diagonal c;
 //    blocks wholly beyond the reach only add to the two end sums.
 //  * ma_dkv_kernel, per 128 keys of a key head: S = Q K^T and dP = dO V^T (a lane holds query rows of ONE key), dV^T += dO^T P, dK^T += Q^T dT over
 //    all query heads of the group.  Where that gives too few blocks, the (head, tile) list is dealt to `nsp` blocks whose fp32 sums are added.
@@ -16,38 +17,7 @@
 
 namespace {
 
-// per row (b, h, i): lse in log2 units (+inf for a row that sees nothing: P = 0), D, and (fp16) amax |dO|; 16 lanes per row
-template <typename T>
-__global__ __launch_bounds__(256) void ma_stat_kernel(const MgldMaskAttn p, float* lse2, float* delta, float* amax, const int64_t rows) {
-  const int sub = threadIdx.x & 15;
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.heads), b = (int)(row / p.Nq / p.heads);
-  typedef typename MaVec<T>::v8 v8;
-  float s = 0.f, m = 0.f;
-  const float lse = p.lse[row];
-  if (sub * 8 < p.head_dim) {
-    const v8 o = *(const v8*)((const T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh + sub * 8);
-    const v8 g = *(const v8*)((const T*)p.dO + b * p.do_sb + (int64_t)i * p.do_si + h * p.do_sh + sub * 8);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      s += (float)o[e] * (float)g[e];
-      m = fmaxf(m, fabsf((float)g[e]));
-    }
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    s += __shfl_xor(s, o, 64);
-    m = fmaxf(m, __shfl_xor(m, o, 64));
-  }
-  if (sub == 0) {
-    lse2[row] = lse == -MA_INF ? MA_INF : lse * MA_LOG2E;
-    delta[row] = lse == -MA_INF ? 0.f : s;
-    if (amax) amax[row] = lse == -MA_INF ? 0.f : m;
-  }
-}
-
-// the largest finite amax of all rows -> out[0]
+// the largest finite amax -> out[0]
 __global__ __launch_bounds__(1024) void ma_amax_kernel(const float* amax, const int64_t rows, float* out) {
   __shared__ float sm[16];
   float m = 0.f;
@@ -71,7 +41,7 @@ __device__ __forceinline__ float ma_pow2_to(const float amax, const int e) {
 }
 
 struct GradWork {
-  float *lse2, *delta, *amax, *gmax, *rel, *kv;
+  float *delta, *amax, *gmax, *rel, *kv;
   const i32x4* doc;
 };
 
@@ -116,14 +86,27 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   const int lim = rok ? bs.limit(p, pos) : 0;
   const int dq = docs && rok ? p.doc_q[b * p.doc_q_sb + i] : -1, dqm = dq < 0 ? -2 : dq;
   const int64_t srow = ((int64_t)b * p.heads + h) * p.Nq + i;
-  const float lse2 = rok ? w.lse2[srow] : MA_INF, delta = rok ? w.delta[srow] : 0.f;
-  const float up = sizeof(T) == 2 && w.amax && rok ? ma_pow2_to(w.amax[srow], 5) : 1.f;      // fp16: dT is rounded as dT * up
+  const float lse = rok ? p.lse[srow] : -MA_INF;
+  const float lse2 = lse == -MA_INF ? MA_INF : lse * MA_LOG2E;          // a row that sees nothing: P = 0
   v8 qf[DK], gf[DK];
 #pragma unroll
   for (int ks = 0; ks < DK; ++ks) {
     const bool ok = rok && lse2 < MA_INF && ks * 2 + lhi < d8;         // a row that sees nothing adds nothing, whatever it holds
     qf[ks] = ok ? *(const v8*)((const T*)p.Q + b * p.q_sb + (int64_t)i * p.q_si + h * p.q_sh + ks * 16 + lhi * 8) : zero;
     gf[ks] = ok ? *(const v8*)((const T*)p.dO + b * p.do_sb + (int64_t)i * p.do_si + h * p.do_sh + ks * 16 + lhi * 8) : zero;
+  }
+  constexpr bool F16 = __is_same(T, f16);
+  float up = 1.f;                                                      // fp16: dT is rounded as dT * up
+  if (F16) {
+    float am = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf((float)gf[ks][e]));
+    am = fmaxf(am, __shfl_xor(am, 32, 64));
+    up = ma_pow2_to(am, 5);
+    am = wave_max(am < MA_INF ? am : 0.f);
+    if (lane == 0) w.amax[(int64_t)blockIdx.x * 4 + wave] = am;
   }
   if (MODE & MA_REL) ma_load_rel(p, h, srel, MA_LOG2E);
   float* const sblk = srel + ((MODE & MA_REL) ? nrel : 0) + wave * (32 * 33 + nrel);
@@ -161,13 +144,68 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     if (docs && wave == 0) ma_dma4(lds0 + 4 * TBYTES + buf * MA_KT * 4, lane, bs.len - k0, ids);
   };
 
+  const int kbase = TL::row_base(lane), tbase = TL::tr_base(lane);
+  // a 32-key half of tile t: scores and dP
+  auto products = [&](const char* sk, const char* sv, const int k2, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    s = ma_zero();
+    dp = ma_zero();
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) s = ma_mfma(TL::template row_frag<v8>(sk, kbase, k2 * 32, ks), qf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) dp = ma_mfma(TL::template row_frag<v8>(sv, kbase, k2 * 32, ks), gf[ks], dp);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int buf = 0;
+  float delta = 0.f;
+  {                                                    // D = sum P dP
+    int fl = 0, fln = 0;
+    int t = advance(fl);
+    if (t >= 0) load_tile(t, buf, fl);
+    while (t >= 0) {
+      ma_dma_wait();
+      __syncthreads();
+      const int tn = advance(fln);
+      if (tn >= 0) load_tile(tn, buf ^ 1, fln);
+      if (fl & 1) {
+        const char* const sk = smem + buf * 2 * TBYTES;
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+          f32x16 s, dp;
+          products(sk, sk + TBYTES, k2, s, dp);
+          const int k0 = t * MA_KT + k2 * 32;
+          const int dl = ma_opaque(k0 + lhi * 4 - pos), ll = ma_opaque(lim - (k0 + lhi * 4));
+#pragma unroll
+          for (int rg = 0; rg < 4; ++rg) {
+            i32x4 dk4 = {dqm, dqm, dqm, dqm};
+            if (docs && !(fl & 2)) dk4 = *(const i32x4*)(sdoc + buf * MA_KT + k2 * 32 + rg * 8 + lhi * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = rg * 4 + e;
+              float sq = 0.f;
+              float x = sc.prob(s[r], dl + rg * 8 + e, lse2, sq) * dp[r];
+              if (!(fl & 2)) x = (rg * 8 + e < ll) & (dk4[e] == dqm) ? x : 0.f;
+              delta += x;
+            }
+          }
+        }
+      }
+      buf ^= 1;
+      t = tn; fl = fln;
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (rok && lhi == 0) w.delta[srow] = delta;
+    __syncthreads();                                   // everyone is done with both buffers
+    w0 = -64;
+    bact = 0;
+  }
+
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = ma_zero();
-  const int kbase = TL::row_base(lane), tbase = TL::tr_base(lane);
-  int fl = 0, fln = 0, buf = 0;
+  int fl = 0, fln = 0;
   int t = advance(fl);
-  if (t >= 0) load_tile(t, 0, fl);
+  if (t >= 0) load_tile(t, buf, fl);
   while (t >= 0) {
     ma_dma_wait();
     __syncthreads();
@@ -178,13 +216,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
       const char* const sv = sk + TBYTES;
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
-        __builtin_amdgcn_sched_barrier(0);
-        f32x16 s = ma_zero(), dp = ma_zero();
-#pragma unroll
-        for (int ks = 0; ks < DK; ++ks) s = ma_mfma(TL::template row_frag<v8>(sk, kbase, k2 * 32, ks), qf[ks], s);
-#pragma unroll
-        for (int ks = 0; ks < DK; ++ks) dp = ma_mfma(TL::template row_frag<v8>(sv, kbase, k2 * 32, ks), gf[ks], dp);
-        __builtin_amdgcn_sched_barrier(0);
+        f32x16 s, dp;
+        products(sk, sv, k2, s, dp);
         const int k0 = t * MA_KT + k2 * 32;
         const int dl = ma_opaque(k0 + lhi * 4 - pos), ll = ma_opaque(lim - (k0 + lhi * 4));
 #pragma unroll
@@ -295,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
   constexpr int DK = D / 16, DT = D / 32, ROWS = D == 64 ? 64 : 32, NH = ROWS / 32;
   constexpr bool VLDS = D == 128;
   constexpr int TBYTES = ROWS * TL::RB, STAT = 3 * MA_KT * 4;
-  extern __shared__ __attribute__((aligned(16))) char smem[];      // [2] x {Q, dO}, [2] x {lse2, delta, doc numbers} [64], D = 128: V of the block's keys; the distance rows
+  extern __shared__ __attribute__((aligned(16))) char smem[];      // [2] x {Q, dO}, [2] x {lse, delta, doc numbers} [64], D = 128: V of the block's keys; the distance rows
   char* const sstat = smem + 4 * TBYTES;
   char* const sV = sstat + 2 * STAT;
   float* const srel = (float*)(sV + (VLDS ? 128 * TL::RB : 0));
@@ -339,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
     const int n = G * (2 * p.reach + 1);
     for (int e = tid; e < n; e += 256) srel[e] = p.rel[(int64_t)hk * n + e] * MA_LOG2E;
   }
-  constexpr bool F16 = sizeof(T) == 2 && __is_same(T, f16);
+  constexpr bool F16 = __is_same(T, f16);
   const float pup = F16 ? 10.f : 0.f;                                // fp16: P is rounded as 2^10 P, dT as 2^6 g dT
   const float gup = F16 ? ma_pow2_to(w.gmax[0], -5) * 0.0625f : 1.f; // (P carries 2^10 already)
 
@@ -387,7 +420,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
     dq.load((const T*)p.Q + b * p.q_sb + h * p.q_sh, (int64_t)i0 * p.q_si * 2, p.q_si, p.Nq - i0, a, flags & 4 ? ids : nullptr);
     dg.load((const T*)p.dO + b * p.do_sb + h * p.do_sh, (int64_t)i0 * p.do_si * 2, p.do_si, p.Nq - i0, a + TBYTES, flags & 4 ? ids : nullptr);
     const int64_t row = ((int64_t)b * p.heads + h) * p.Nq + i0;
-    if (wave == 0) ma_dma4(st, lane, p.Nq - i0, w.lse2 + row);
+    if (wave == 0) ma_dma4(st, lane, p.Nq - i0, p.lse + row);
     if (wave == 1) ma_dma4(st + 256, lane, p.Nq - i0, w.delta + row);
     if (wave == 2 && docs) ma_dma4(st + 512, lane, p.Nq - i0, ids);
   };
@@ -428,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
           const int rr = q2 * 32 + rg * 8 + lhi * 4;
-          const f32x4 lse2 = *(const f32x4*)(sl + rr), delta = *(const f32x4*)(sl + 64 + rr);
+          const f32x4 lse2 = *(const f32x4*)(sl + rr) * MA_LOG2E, delta = *(const f32x4*)(sl + 64 + rr);
           i32x4 di = {dj, dj, dj, dj};
           if (docs && !(fl & 2)) di = *(const i32x4*)((const int*)sl + 128 + rr);
 #pragma unroll
@@ -520,7 +553,7 @@ __global__ __launch_bounds__(256) void ma_kv_sum_kernel(const MgldMaskAttn p, co
 int64_t up256(const int64_t n) { return (n + 255) / 256 * 256; }
 struct GradPlan {
   int nsp, nqb, nkb;
-  int64_t rows, doc, lse2, delta, amax, gmax, rel, kv, total;      // byte offsets
+  int64_t rows, doc, delta, amax, gmax, rel, kv, total;      // byte offsets
 };
 GradPlan grad_plan(const MgldMaskAttn* p) {
   GradPlan g;
@@ -533,10 +566,9 @@ GradPlan grad_plan(const MgldMaskAttn* p) {
   if (n > (items + 3) / 4) n = (items + 3) / 4;
   g.nsp = n < 1 ? 1 : n > 8 ? 8 : (int)n;
   g.doc = 0;
-  g.lse2 = up256(ma_doc_bytes(p));
-  g.delta = g.lse2 + up256(g.rows * 4);
+  g.delta = up256(ma_doc_bytes(p));
   g.amax = g.delta + up256(g.rows * 4);
-  g.gmax = g.amax + (p->bf16 ? 0 : up256(g.rows * 4));
+  g.gmax = g.amax + (p->bf16 ? 0 : up256((int64_t)p->batch * p->heads * g.nqb * 16));
   g.rel = g.gmax + 256;
   g.kv = g.rel + (p->dRel ? up256(g.rows ? (int64_t)p->batch * p->heads * g.nqb * (2 * p->reach + 1) * 4 : 0) : 0);
   g.total = g.kv + (g.nsp > 1 ? (int64_t)g.nsp * p->batch * p->Nkv * p->kv_heads * 2 * D * 4 : 0);
@@ -554,22 +586,19 @@ int grad_launch(const MgldMaskAttn& p, hipStream_t st) {
   char* const wk = (char*)p.work;
   GradWork w;
   w.doc = (const i32x4*)(wk + g.doc);
-  w.lse2 = (float*)(wk + g.lse2);
   w.delta = (float*)(wk + g.delta);
   w.amax = p.bf16 ? nullptr : (float*)(wk + g.amax);
   w.gmax = (float*)(wk + g.gmax);
   w.rel = (float*)(wk + g.rel);
   w.kv = (float*)(wk + g.kv);
   const int nrel = p.rel ? 2 * p.reach + 1 : 0, G = p.heads / p.kv_heads;
-  MGLD_REQUIRE(g.rows <= (int64_t)0x7fffffff * 16 && (int64_t)g.nqb * p.batch * p.heads <= 0x7fffffff && (int64_t)g.nkb * p.batch * p.kv_heads * g.nsp <= 0x7fffffff,
+  MGLD_REQUIRE((int64_t)g.nqb * p.batch * p.heads <= 0x7fffffff && (int64_t)g.nkb * p.batch * p.kv_heads * g.nsp <= 0x7fffffff,
                "masked_attention_grad: grid");
   if (p.doc_q) {
     const int rc = ma_doc_tiles(p, wk + g.doc, st);
     if (rc) return rc;
   }
   if (p.Nq > 0) {
-    ma_stat_kernel<T><<<dim3((unsigned)((g.rows + 15) / 16)), 256, 0, st>>>(p, w.lse2, w.delta, w.amax, g.rows);
-    if (w.amax) ma_amax_kernel<<<1, 1024, 0, st>>>(w.amax, g.rows, w.gmax);
     const dim3 grid((unsigned)((int64_t)g.nqb * p.batch * p.heads));
     const int lds = 4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + nrel * 4;
     if constexpr (MODE & MA_REL) {
@@ -583,7 +612,8 @@ int grad_launch(const MgldMaskAttn& p, hipStream_t st) {
       grad_lds(ma_dq_kernel<T, D, MODE, false>, lds);
       ma_dq_kernel<T, D, MODE, false><<<grid, 256, lds, st>>>(p, w, g.nqb);
     }
-  } else if (w.amax) ma_amax_kernel<<<1, 1024, 0, st>>>(w.amax, 0, w.gmax);
+  }
+  if (w.amax) ma_amax_kernel<<<1, 1024, 0, st>>>(w.amax, (int64_t)p.batch * p.heads * g.nqb * 4, w.gmax);
   if (p.dRel) ma_rel_sum_kernel<<<dim3(cdiv(nrel, 256), p.heads), 256, 0, st>>>(w.rel, p.dRel, p.batch, p.heads, g.nqb, nrel);
   if (p.Nkv > 0) {
     constexpr int ROWS = D == 64 ? 64 : 32;

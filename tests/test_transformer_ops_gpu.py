@@ -4,7 +4,7 @@ Tolerances are error bounds, element by element.  With u half a step of the type
 fp32 score (E = 2 (scale sum|q k| (d + 4) 2^-24 + 2^-20 softcap + 2^-20), two of them: numerator and normaliser):
   o   : u |o| + (u + E) sum P |v|                       (one rounding of the result, one of every probability)
   dv  : u |dv| + (u + E) sum P |do|
-  dS  : P (d 2^-24 sum|do v| + sum |do| tol(o)) + E |dS|     (D = do.o uses the rounded o)
+  dS  : P (d 2^-24 sum|do v| + tol(D)) + E |dS|,  tol(D) = sum P (d 2^-24 sum|do v| + E |dP|)
   dq  : u |dq| + scale sum (u |dT| + tol(dS)) |k|;  dk likewise with |q|;  drel: sum tol(dS) + 2^-14 sum |dS|
 and for fp16 what the smallest step of the scaled operands leaves.
 """
@@ -259,8 +259,8 @@ def reference(q, k, v, do, kw, grads=True):
         dP = torch.matmul(dob, vv.permute(0, 2, 3, 1))
         D = (do64 * r["o"]).sum(-1).permute(0, 2, 1)[..., None]
         dS = P * (dP - D)
-        tD = (do64.abs() * to).sum(-1).permute(0, 2, 1)[..., None]
         tdP = torch.matmul(dob.abs(), vv.abs().permute(0, 2, 3, 1)) * (d + 4) * 2.0 ** -24
+        tD = (P * (tdP + E * dP.abs())).sum(-1, keepdim=True) * 1.02
         tS = P * (tdP + tD) + E * (dS.abs() + P * tD)
         f = 1 - (r["u"] / cap) ** 2 if cap else torch.ones_like(dS)
         dT = dS * f
