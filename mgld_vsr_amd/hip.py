@@ -5,6 +5,7 @@ and dtype bookkeeping.  Every compute call goes through the C ABI; if the librar
 this module's `lib()` fails loudly — there is no eager/CPU fallback on the product path.
 """
 import ctypes as C
+import functools
 import threading
 import os
 
@@ -947,29 +948,32 @@ def hp_softmax_rows(S):
 # dimension.  There is no autograd: the gradient is its own call.  Results the caller does not pass are allocated; while a graph is being
 # captured they and `work` have to be passed (memory handed back to torch's allocator would be reused under the graph).  Two calls whose work
 # may overlap in time (two streams, two captured graphs) need work buffers of their own.
-class _OnDevice:
-    """makes the tensors' device the current one for a call (the launch goes to its current stream)"""
-
-    def __init__(self, t):
-        self.dev = t.device
-
-    def __enter__(self):
-        self.ctx = None
-        if self.dev.index is not None and self.dev.index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(self.dev)
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
+def _on_its_device(fn):
+    """runs fn with its first tensor's device as the current one (the launch goes to that device's current stream)"""
+    @functools.wraps(fn)
+    def call(*a, **kw):
+        for t in (a or kw.values()):
+            if t is not None:
+                break
+        else:
+            t = None
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(t.get_device()):
+                return fn(*a, **kw)
+        return fn(*a, **kw)
+    return call
 
 
 def _same_device(what, *ts):
     _req_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if not (len(devs) <= 1):
-        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devs))}")
+    dev = None
+    for t in ts:
+        if t is not None:
+            d = t.get_device()
+            if dev is None:
+                dev = d
+            elif d != dev:
+                raise ValueError(f"{what}: tensors on different devices")
 
 
 class _Memory:
@@ -996,35 +1000,34 @@ def _overlap(a, b):
 
 
 def _same_view(a, b):
-    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and _strides(a) == _strides(b)
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
 
-def _strides(t):
-    """strides but the last one's; a dimension of one element has none"""
-    return tuple(0 if n == 1 else st for n, st in zip(t.shape[:-1], t.stride()[:-1]))
-
-
-def _heads_view(what, name, t, dim, dtype=None, shape=None):
+def _view(what, name, t, dim, dtype=None, shape=None):
+    """checks a [.., heads, d] tensor; its strides but the last one's (a dimension of one element has none)"""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what}: {name} must be a tensor")
-    if not (t.dtype in (torch.float16, torch.bfloat16)):
-        raise ValueError(f"{what}: {name} must be float16 or bfloat16, got {t.dtype}")
-    if not (dtype is None or t.dtype == dtype):
-        raise ValueError(f"{what}: {name} is {t.dtype}, the call is {dtype}")
-    if not (t.dim() == dim and (t.shape[-1] <= 1 or t.stride(-1) == 1)):
-        raise ValueError(f"{what}: {name} must have {dim} dimensions and unit stride along the last, got {tuple(t.shape)} {t.stride()}")
-    if not (shape is None or tuple(t.shape) == tuple(shape)):
-        raise ValueError(f"{what}: {name} must be {shape}, got {tuple(t.shape)}")
+    dt, sh = t.dtype, t.shape
+    if dt is not dtype and (dtype is not None or (dt is not torch.float16 and dt is not torch.bfloat16)):
+        raise ValueError(f"{what}: {name} must be {dtype or 'float16 or bfloat16'}, got {dt}")
+    if shape is not None and sh != shape:
+        raise ValueError(f"{what}: {name} must be {tuple(shape)}, got {tuple(sh)}")
+    st = t.stride()
+    if len(sh) != dim or (st[-1] != 1 and sh[-1] > 1):
+        raise ValueError(f"{what}: {name} must have {dim} dimensions and unit stride along the last, got {tuple(sh)} {st}")
+    if dim == 3:
+        return st[0] if sh[0] != 1 else 0, st[1] if sh[1] != 1 else 0
+    return st[0] if sh[0] != 1 else 0, st[1] if sh[1] != 1 else 0, st[2] if sh[2] != 1 else 0
 
 
 def _out(what, name, t, like, capturing, inputs=(), inplace=(), shape=None, dtype=None):
     """an output the caller passed (checked) or a new one"""
-    shape, dtype = tuple(like.shape if shape is None else shape), like.dtype if dtype is None else dtype
     if t is None:
         if capturing:
             raise ValueError(f"{what}: pass {name}= while a graph is being captured")
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if not (tuple(t.shape) == shape and t.dtype == dtype and t.device == like.device):
+        return torch.empty_like(like) if shape is None else torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
+    shape, dtype = tuple(like.shape if shape is None else shape), like.dtype if dtype is None else dtype
+    if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == like.device):
         raise ValueError(f"{what}: {name} must be {dtype} {shape} on {like.device}")
     if not (t.numel() == 0 or all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride()))):
         raise ValueError(f"{what}: {name} must not repeat its elements")
@@ -1035,12 +1038,9 @@ def _out(what, name, t, like, capturing, inputs=(), inplace=(), shape=None, dtyp
     return t
 
 
-def _vec(what, name, t, n, dtype, like):
-    if t is not None:
-        if not (isinstance(t, torch.Tensor) and t.dtype == dtype and tuple(t.shape) == n and t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be contiguous {dtype} {n}")
-        if not (t.device == like.device):
-            raise ValueError(f"{what}: {name} must be on {like.device}")
+def _vec(what, name, t, shape, dtype):
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous {dtype} {shape}")
     return t
 
 
@@ -1073,69 +1073,62 @@ def rope_freqs(rot_dim, base=10000.0, device="cuda"):
     return base ** (-2.0 * torch.arange(rot_dim // 2, dtype=torch.float64, device=device) / max(1, rot_dim))
 
 
-def _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps, interleaved):
-    for n, t in (("q", q), ("k", k)):
-        if t is not None:
-            _heads_view(what, n, t, 3)
+def _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps):
+    """(type, rows, head size, rot_dim, pos is int64, strides of q and k)"""
     x = q if q is not None else k
-    if not (x is not None):
+    if x is None:
         raise ValueError(f"{what}: q or k")
-    rows, d = x.shape[0], x.shape[2]
-    for n, t in (("q", q), ("k", k)):
-        if t is not None:
-            if not (t.dtype == x.dtype and t.shape[0] == rows and t.shape[2] == d):
-                raise ValueError(f"{what}: q and k must agree in type, rows and head size")
+    sq = _view(what, "q", q, 3) if q is not None else None
+    sk = _view(what, "k", k, 3, x.dtype) if k is not None else None
+    rows, _, d = x.shape
+    if k is not None and (k.shape[0] != rows or k.shape[2] != d):
+        raise ValueError(f"{what}: q and k must agree in rows and head size")
     _same_device(what, q, k, pos, freqs, q_gamma, k_gamma)
-    if not (d % 8 == 0 and 8 <= d <= 256):
+    if d % 8 or not 8 <= d <= 256:
         raise ValueError(f"{what}: head size {d}: a multiple of 8 up to 256")
-    rot = 0
+    rot = p64 = 0
     if freqs is not None:
-        if not (freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous()):
+        if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
             raise ValueError(f"{what}: freqs must be contiguous float64 [rot_dim / 2]")
         rot = 2 * freqs.shape[0]
-        if not (rot <= d and rot % 8 == 0):
+        if rot > d or rot % 8:
             raise ValueError(f"{what}: rot_dim {rot}: a multiple of 8 up to the head size")
     if rot:
-        if not (pos is not None and pos.dtype in (torch.int32, torch.int64) and tuple(pos.shape) == (rows,) and pos.is_contiguous()):
+        p64 = pos is not None and pos.dtype is torch.int64
+        if pos is None or not (p64 or pos.dtype is torch.int32) or pos.shape != (rows,) or not pos.is_contiguous():
             raise ValueError(f"{what}: pos must be contiguous int32 or int64 [{rows}]")
-    _vec(what, "q_gamma", q_gamma, (d,), torch.float32, x)
-    _vec(what, "k_gamma", k_gamma, (d,), torch.float32, x)
-    if not (eps >= 0):
+    for n, g in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+        if g is not None:
+            _vec(what, n, g, (d,), torch.float32)
+    if not eps >= 0:
         raise ValueError(f"{what}: eps must not be negative")
-    p = MgldQkRope()
-    p.rows, p.head_dim, p.rot_dim, p.interleaved, p.bf16, p.eps = rows, d, rot, int(bool(interleaved)), int(x.dtype == torch.bfloat16), eps
-    if rot:
-        p.pos, p.freqs, p.pos64 = pos.data_ptr(), freqs.data_ptr(), int(pos.dtype == torch.int64)
-    return p, x
+    return x, rows, d, rot, int(p64), sq, sk
 
 
-def _side(h, x, y, dy=None, gamma=None, dgamma=None):
-    h.heads = x.shape[1]
-    h.x, (h.x_sr, h.x_sh) = x.data_ptr(), _strides(x)
-    h.y, (h.y_sr, h.y_sh) = y.data_ptr(), _strides(y)
-    if dy is not None:
-        h.dy, (h.dy_sr, h.dy_sh) = dy.data_ptr(), _strides(dy)
-    h.gamma, h.dgamma = _p(gamma).value, _p(dgamma).value
+_NO_HEADS = (None, None, None, None, None, 0, 0, 0, 0, 0, 0, 0)
 
 
+@_on_its_device
 def qk_norm_rope(q, k, pos, freqs, *, q_gamma=None, k_gamma=None, eps=1e-6, interleaved=False, q_out=None, k_out=None):
     """Root-mean-square norm of every query and key head and the rotation of its first 2 * len(freqs) elements, one pass (include/mgld_hip.h).
     q [rows, heads, d], k [rows, kv_heads, d] (either may be None); pos int32 / int64 [rows]; freqs float64 (rope_freqs; None: no rotation);
     gammas fp32 [d].  q_out / k_out may be q / k themselves.  -> (q_out, k_out)"""
     what = "qk_norm_rope"
-    p, x = _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps, interleaved)
-    with _OnDevice(x):
-        cap = _capturing()
-        ins = (q, k, pos, freqs, q_gamma, k_gamma)
-        if q is not None:
-            q_out = _out(what, "q_out", q_out, q, cap, ins, (q,))
-            _heads_view(what, "q_out", q_out, 3)
-            _side(p.q, q, q_out, gamma=q_gamma)
-        if k is not None:
-            k_out = _out(what, "k_out", k_out, k, cap, ins + (q_out,), (k,))
-            _heads_view(what, "k_out", k_out, 3)
-            _side(p.k, k, k_out, gamma=k_gamma)
-        _chk(lib().mgld_qk_norm_rope(C.byref(p), stream_ptr()), what)
+    x, rows, d, rot, p64, sq, sk = _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps)
+    cap = _capturing()
+    ins = (q, k, pos, freqs, q_gamma, k_gamma)
+    hq = hk = _NO_HEADS
+    if q is not None:
+        q_out = _out(what, "q_out", q_out, q, cap, ins, (q,))
+        hq = (q.data_ptr(), q_out.data_ptr(), None, q_gamma.data_ptr() if q_gamma is not None else None, None, *sq,
+              *_view(what, "q_out", q_out, 3), 0, 0, q.shape[1])
+    if k is not None:
+        k_out = _out(what, "k_out", k_out, k, cap, ins + (q_out,), (k,))
+        hk = (k.data_ptr(), k_out.data_ptr(), None, k_gamma.data_ptr() if k_gamma is not None else None, None, *sk,
+              *_view(what, "k_out", k_out, 3), 0, 0, k.shape[1])
+    p = MgldQkRope(hq, hk, pos.data_ptr() if rot else None, freqs.data_ptr() if rot else None, None, 0, rows, p64, d, rot, 1 if interleaved else 0,
+                   x.dtype is torch.bfloat16, eps)
+    _chk(lib().mgld_qk_norm_rope(C.byref(p), stream_ptr()), what)
     return (q_out if q is not None else None), (k_out if k is not None else None)
 
 
@@ -1145,104 +1138,105 @@ def qk_norm_rope_grad_work_bytes(rows, head_dim):
     return int(lib().mgld_qk_norm_rope_grad_work(C.byref(p)))
 
 
+@_on_its_device
 def qk_norm_rope_grad(q, k, pos, freqs, dq_out, dk_out, *, q_gamma=None, k_gamma=None, eps=1e-6, interleaved=False, dq=None, dk=None,
                       dq_gamma=None, dk_gamma=None, work=None):
     """Gradient of qk_norm_rope: q, k are ITS inputs, dq_out / dk_out the gradients of its results.  -> (dq, dk, dq_gamma, dk_gamma); a gamma's
     gradient is fp32 [d], None where that gamma is.  dq may be dq_out or q (dk likewise)."""
     what = "qk_norm_rope_grad"
-    p, x = _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps, interleaved)
-    if not ((q is None) == (dq_out is None) and (k is None) == (dk_out is None)):
+    x, rows, d, rot, p64, sq, sk = _qk_rope(what, q, k, pos, freqs, q_gamma, k_gamma, eps)
+    if (q is None) != (dq_out is None) or (k is None) != (dk_out is None):
         raise ValueError(f"{what}: a gradient for each of q, k")
     _same_device(what, x, dq_out, dk_out)
-    with _OnDevice(x):
-        cap = _capturing()
-        ins = (q, k, pos, freqs, q_gamma, k_gamma, dq_out, dk_out)
-        outs = []
-        for n, t, g, gamma, dt, dg, side in (("q", q, dq_out, q_gamma, dq, dq_gamma, p.q), ("k", k, dk_out, k_gamma, dk, dk_gamma, p.k)):
-            if t is None:
-                outs += [None, None]
-                continue
-            _heads_view(what, f"d{n}_out", g, 3, x.dtype, t.shape)
-            dt = _out(what, "d" + n, dt, t, cap, ins + tuple(outs), (t, g))
-            _heads_view(what, "d" + n, dt, 3)
-            outs.append(dt)
-            if gamma is not None:
-                dg = _out(what, f"d{n}_gamma", dg, gamma, cap, ins + tuple(outs))
-                if not dg.is_contiguous():
-                    raise ValueError(f"{what}: d{n}_gamma must be contiguous")
-            else:
-                dg = None
-            outs.append(dg)
-            _side(side, t, dt, g, gamma, dg)
-        if outs[1] is not None or outs[3] is not None:
-            work = _work(what, work, int(lib().mgld_qk_norm_rope_grad_work(C.byref(p))), x, cap, ins + tuple(outs))
-            _set_work(p, work)
-        _chk(lib().mgld_qk_norm_rope_grad(C.byref(p), stream_ptr()), what)
+    cap = _capturing()
+    ins = (q, k, pos, freqs, q_gamma, k_gamma, dq_out, dk_out)
+    outs, sides = [], []
+    for n, t, st, g, gamma, dt, dg in (("q", q, sq, dq_out, q_gamma, dq, dq_gamma), ("k", k, sk, dk_out, k_gamma, dk, dk_gamma)):
+        if t is None:
+            outs += [None, None]
+            sides.append(_NO_HEADS)
+            continue
+        sg = _view(what, f"d{n}_out", g, 3, x.dtype, t.shape)
+        dt = _out(what, "d" + n, dt, t, cap, ins + tuple(outs), (t, g))
+        outs.append(dt)
+        if gamma is not None:
+            dg = _out(what, f"d{n}_gamma", dg, gamma, cap, ins + tuple(outs))
+            if not dg.is_contiguous():
+                raise ValueError(f"{what}: d{n}_gamma must be contiguous")
+        else:
+            dg = None
+        outs.append(dg)
+        sides.append((t.data_ptr(), dt.data_ptr(), g.data_ptr(), gamma.data_ptr() if gamma is not None else None, dg.data_ptr() if dg is not None else None,
+                      *st, *_view(what, "d" + n, dt, 3), *sg, t.shape[1]))
+    p = MgldQkRope(*sides, pos.data_ptr() if rot else None, freqs.data_ptr() if rot else None, None, 0, rows, p64, d, rot, 1 if interleaved else 0,
+                   x.dtype is torch.bfloat16, eps)
+    if outs[1] is not None or outs[3] is not None:
+        work = _work(what, work, lib().mgld_qk_norm_rope_grad_work(C.byref(p)), x, cap, ins + tuple(outs))
+        _set_work(p, work)
+    _chk(lib().mgld_qk_norm_rope_grad(C.byref(p), stream_ptr()), what)
     return outs[0], outs[2], outs[1], outs[3]
 
 
 def _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0):
-    """the checked problem without outputs"""
-    _heads_view(what, "q", q, 4)
-    _heads_view(what, "k", k, 4, q.dtype)
-    _heads_view(what, "v", v, 4, q.dtype, k.shape)
+    """the checked problem without its results: (tensors it reads, values of MgldMaskAttn's fields by group)"""
+    sq = _view(what, "q", q, 4)
+    sk = _view(what, "k", k, 4, q.dtype)
+    sv = _view(what, "v", v, 4, q.dtype, k.shape)
     B, Nq, H, d = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    if not (k.shape[0] == B and k.shape[3] == d):
+    Bk, Nk, Hk, dk = k.shape
+    if Bk != B or dk != d:
         raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch and head size")
-    if not (Hk > 0 and H > 0 and H % Hk == 0):
+    if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{what}: {H} query heads over {Hk} key heads")
-    if not (d % 8 == 0 and 8 <= d <= 128):
+    if d % 8 or not 8 <= d <= 128:
         raise ValueError(f"{what}: head size {d}: a multiple of 8 up to 128")
-    _same_device(what, q, k, v, slopes, rel, prefix, kv_len)
-    scale = float(d) ** -0.5 if scale is None else float(scale)
+    scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap or 0.0)
     if not (0.0 < scale < 3e38 and 0.0 <= softcap < 3e38):
         raise ValueError(f"{what}: scale must be positive, softcap not negative")
-    if not (slopes is None or rel is None):
-        raise ValueError(f"{what}: slopes or rel, not both")
-    p = MgldMaskAttn()
-    p.batch, p.heads, p.kv_heads, p.Nq, p.Nkv, p.head_dim = B, H, Hk, Nq, Nk, d
-    p.bf16, p.causal, p.scale, p.softcap = int(q.dtype == torch.bfloat16), int(bool(causal)), scale, softcap
-    p.slopes = _p(_vec(what, "slopes", slopes, (H,), torch.float32, q)).value
+    ins = [q, k, v]
+    ptr = [None] * 6
+    reach = dqs = dks = 0
+    if slopes is not None:
+        if rel is not None:
+            raise ValueError(f"{what}: slopes or rel, not both")
+        ptr[0] = _vec(what, "slopes", slopes, (H,), torch.float32).data_ptr()
+        ins.append(slopes)
     if rel is not None:
-        if not (rel.dim() == 2 and rel.shape[1] % 2 == 1 and rel.shape[1] <= 2049):
+        if rel.dim() != 2 or rel.shape[1] % 2 != 1 or rel.shape[1] > 2049:
             raise ValueError(f"{what}: rel must be [heads, 2 * reach + 1] with reach up to 1024")
-        _vec(what, "rel", rel, (H, rel.shape[1]), torch.float32, q)
-        p.rel, p.reach = rel.data_ptr(), rel.shape[1] // 2
+        ptr[1], reach = _vec(what, "rel", rel, (H, rel.shape[1]), torch.float32).data_ptr(), rel.shape[1] // 2
+        ins.append(rel)
     if docs is not None:
         if isinstance(docs, torch.Tensor):
-            if not (Nq == Nk):
+            if Nq != Nk:
                 raise ValueError(f"{what}: one docs tensor needs as many queries as keys; pass (doc_q, doc_k)")
             docs = (docs, docs)
         for n, t, m in (("doc_q", docs[0], Nq), ("doc_k", docs[1], Nk)):
-            if not (t.dtype == torch.int32 and tuple(t.shape) == (B, m) and (m <= 1 or t.stride(1) == 1)):
+            if t.dtype is not torch.int32 or t.shape != (B, m) or (m > 1 and t.stride(1) != 1):
                 raise ValueError(f"{what}: {n} must be int32 [{B}, {m}] with unit stride")
-        _same_device(what, q, *docs)
-        p.doc_q, p.doc_k = docs[0].data_ptr() or None, docs[1].data_ptr() or None
-        p.doc_q_sb, p.doc_k_sb = _strides(docs[0])[0], _strides(docs[1])[0]
-    if not (prefix is None or causal):
-        raise ValueError(f"{what}: prefix needs causal=True")
-    p.prefix = _p(_vec(what, "prefix", prefix, (B,), torch.int32, q)).value
-    p.kv_len = _p(_vec(what, "kv_len", kv_len, (B,), torch.int32, q)).value
-    if q_pos0 is None:
-        p.q_from_end = 1
-    else:
-        if not (abs(int(q_pos0)) <= 1 << 30):
-            raise ValueError(f"{what}: q_pos0")
-        p.q_pos0 = int(q_pos0)
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        _put(p, n, n.upper(), t)
-    ins = (q, k, v, slopes, rel, prefix, kv_len) + (tuple(docs) if docs is not None else ())
-    return p, ins
+        ptr[2], ptr[3] = docs[0].data_ptr() or None, docs[1].data_ptr() or None
+        dqs, dks = docs[0].stride(0) if B > 1 else 0, docs[1].stride(0) if B > 1 else 0
+        ins += docs
+    if prefix is not None:
+        if not causal:
+            raise ValueError(f"{what}: prefix needs causal=True")
+        ptr[4] = _vec(what, "prefix", prefix, (B,), torch.int32).data_ptr()
+        ins.append(prefix)
+    if kv_len is not None:
+        ptr[5] = _vec(what, "kv_len", kv_len, (B,), torch.int32).data_ptr()
+        ins.append(kv_len)
+    _same_device(what, *ins)
+    if q_pos0 is not None and abs(int(q_pos0)) > 1 << 30:
+        raise ValueError(f"{what}: q_pos0")
+    tail = (B, H, Hk, Nq, Nk, d, reach, 0 if q_pos0 is None else int(q_pos0), q_pos0 is None, 1 if causal else 0, q.dtype is torch.bfloat16, scale, softcap)
+    return ins, sq + sk + sv, ptr, (dqs, dks), tail
 
 
-def _put(p, n, field, t):
-    setattr(p, field, t.data_ptr())
-    for a, st in zip(("_sb", "_si", "_sh"), _strides(t)):
-        setattr(p, n + a, st)
+_NO_GRAD = (None,) * 5 + (0,) * 12
 
 
+@_on_its_device
 def masked_attention(q, k, v, *, scale=None, causal=False, softcap=0.0, slopes=None, rel=None, docs=None, prefix=None, kv_len=None, q_pos0=None,
                      o=None, lse=None, work=None):
     """softmax(scores) v with capped scores, a distance bias and masks (include/mgld_hip.h has the formula).
@@ -1254,23 +1248,24 @@ def masked_attention(q, k, v, *, scale=None, causal=False, softcap=0.0, slopes=N
     q_pos0: position of the first query; None: the queries are the last ones before kv_len (of a cache's newest tokens).
     A query that sees nothing gives 0 (lse -inf).  -> (o like q, lse fp32 [B, heads, Nq])"""
     what = "masked_attention"
-    p, ins = _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
-    B, Nq, H, d = q.shape
-    with _OnDevice(q):
-        cap = _capturing()
-        o = _out(what, "o", o, q, cap, ins)
-        _heads_view(what, "o", o, 4)
-        _put(p, "o", "O", o)
-        lse = _out(what, "lse", lse, q, cap, ins + (o,), shape=(B, H, Nq), dtype=torch.float32)
-        if not lse.is_contiguous():
-            raise ValueError(f"{what}: lse must be contiguous")
-        p.lse = lse.data_ptr()
-        work = _work(what, work, int(lib().mgld_masked_attention_work(C.byref(p))), q, cap, ins + (o, lse))
+    ins, strides, ptr, doc_sb, tail = _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
+    cap = _capturing()
+    o = _out(what, "o", o, q, cap, ins)
+    so = _view(what, "o", o, 4)
+    lse = _out(what, "lse", lse, q, cap, ins + [o], shape=(tail[0], tail[1], tail[3]), dtype=torch.float32)
+    if not lse.is_contiguous():
+        raise ValueError(f"{what}: lse must be contiguous")
+    p = MgldMaskAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), *strides, *so, *ptr, *doc_sb, *_NO_GRAD, None, 0, *tail)
+    L, ref = lib(), C.byref(p)
+    need = L.mgld_masked_attention_work(ref)
+    if need:
+        work = _work(what, work, need, q, cap, ins + [o, lse])
         _set_work(p, work)
-        _chk(lib().mgld_masked_attention(C.byref(p), stream_ptr()), what)
+    _chk(L.mgld_masked_attention(ref, stream_ptr()), what)
     return o, lse
 
 
+@_on_its_device
 def masked_attention_grad(q, k, v, o, lse, do, *, scale=None, causal=False, softcap=0.0, slopes=None, rel=None, docs=None, prefix=None, kv_len=None,
                           q_pos0=None, dq=None, dk=None, dv=None, drel=None, work=None):
     """Gradient of masked_attention, called with the same options, its results o and lse, and do = the gradient of o.  (do . o is summed again
@@ -1278,36 +1273,34 @@ def masked_attention_grad(q, k, v, o, lse, do, *, scale=None, causal=False, soft
     -> (dq, dk, dv, drel): dk / dv summed over the query heads that share them, zeros where no query sees the key; drel fp32 like rel (None
     without rel).  Sums have a fixed order: equal calls give equal bits."""
     what = "masked_attention_grad"
-    p, ins = _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
-    B, Nq, H, d = q.shape
-    _heads_view(what, "o", o, 4, q.dtype, q.shape)
-    _heads_view(what, "do", do, 4, q.dtype, q.shape)
+    ins, strides, ptr, doc_sb, tail = _mask_attn(what, q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
+    so = _view(what, "o", o, 4, q.dtype, q.shape)
+    sdo = _view(what, "do", do, 4, q.dtype, q.shape)
     _same_device(what, q, o, lse, do)
-    _vec(what, "lse", lse, (B, H, Nq), torch.float32, q)
-    ins = ins + (o, lse, do)
-    with _OnDevice(q):
-        cap = _capturing()
-        _put(p, "o", "O", o)
-        _put(p, "do", "dO", do)
-        p.lse = lse.data_ptr()
-        outs = []
-        for n, t, like in (("q", dq, q), ("k", dk, k), ("v", dv, v)):
-            t = _out(what, "d" + n, t, like, cap, ins + tuple(outs))
-            _heads_view(what, "d" + n, t, 4)
-            _put(p, "d" + n, "d" + n.upper(), t)
-            outs.append(t)
-        if rel is not None:
-            drel = _out(what, "drel", drel, rel, cap, ins + tuple(outs))
-            if not drel.is_contiguous():
-                raise ValueError(f"{what}: drel must be contiguous")
-            p.dRel = drel.data_ptr()
-            outs.append(drel)
-        else:
-            outs.append(None)
-        work = _work(what, work, int(lib().mgld_masked_attention_grad_work(C.byref(p))), q, cap, ins + tuple(outs))
+    _vec(what, "lse", lse, (tail[0], tail[1], tail[3]), torch.float32)
+    ins += [o, lse, do]
+    cap = _capturing()
+    dq = _out(what, "dq", dq, q, cap, ins)
+    dk = _out(what, "dk", dk, k, cap, ins + [dq])
+    dv = _out(what, "dv", dv, v, cap, ins + [dq, dk])
+    outs = [dq, dk, dv]
+    if rel is not None:
+        drel = _out(what, "drel", drel, rel, cap, ins + outs)
+        if not drel.is_contiguous():
+            raise ValueError(f"{what}: drel must be contiguous")
+        outs.append(drel)
+    else:
+        drel = None
+    p = MgldMaskAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), *strides, *so, *ptr, *doc_sb, do.data_ptr(), dq.data_ptr(),
+                     dk.data_ptr(), dv.data_ptr(), drel.data_ptr() if drel is not None else None, *sdo, *_view(what, "dq", dq, 4), *_view(what, "dk", dk, 4),
+                     *_view(what, "dv", dv, 4), None, 0, *tail)
+    L, ref = lib(), C.byref(p)
+    need = L.mgld_masked_attention_grad_work(ref)
+    if need:
+        work = _work(what, work, need, q, cap, ins + outs)
         _set_work(p, work)
-        _chk(lib().mgld_masked_attention_grad(C.byref(p), stream_ptr()), what)
-    return tuple(outs)
+    _chk(L.mgld_masked_attention_grad(ref, stream_ptr()), what)
+    return dq, dk, dv, drel
 
 
 class RelBuckets:
@@ -1349,31 +1342,31 @@ def rel_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
     return RelBuckets(num_buckets, max_distance, bool(bidirectional), device)
 
 
+@_on_its_device
 def rel_bias(table, plan, out=None):
     """learned bias table fp32 [buckets, heads] -> fp32 [heads, 2 * reach + 1], the `rel` of masked_attention"""
     what = "rel_bias"
     _same_device(what, table, plan.index)
     if not (table.dim() == 2):
         raise ValueError(f"{what}: table must be [buckets, heads]")
-    _vec(what, "table", table, (plan.num_buckets, table.shape[1]), torch.float32, table)
-    with _OnDevice(table):
-        out = _out(what, "out", out, table, _capturing(), (table, plan.index), shape=(table.shape[1], 2 * plan.reach + 1))
-        if not out.is_contiguous():
-            raise ValueError(f"{what}: out must be contiguous")
-        _chk(lib().mgld_rel_bias(_p(table), _p(plan.index), _p(out), plan.num_buckets, table.shape[1], 2 * plan.reach + 1, stream_ptr()), what)
+    _vec(what, "table", table, (plan.num_buckets, table.shape[1]), torch.float32)
+    out = _out(what, "out", out, table, _capturing(), (table, plan.index), shape=(table.shape[1], 2 * plan.reach + 1))
+    if not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous")
+    _chk(lib().mgld_rel_bias(_p(table), _p(plan.index), _p(out), plan.num_buckets, table.shape[1], 2 * plan.reach + 1, stream_ptr()), what)
     return out
 
 
+@_on_its_device
 def rel_bias_grad(drel, plan, out=None):
     """gradient of rel_bias: drel fp32 [heads, 2 * reach + 1] -> the table's, fp32 [buckets, heads]"""
     what = "rel_bias_grad"
     _same_device(what, drel, plan.index)
     if not (drel.dim() == 2):
         raise ValueError(f"{what}: drel must be [heads, 2 * reach + 1]")
-    _vec(what, "drel", drel, (drel.shape[0], 2 * plan.reach + 1), torch.float32, drel)
-    with _OnDevice(drel):
-        out = _out(what, "out", out, drel, _capturing(), (drel, plan.index), shape=(plan.num_buckets, drel.shape[0]))
-        if not out.is_contiguous():
-            raise ValueError(f"{what}: out must be contiguous")
-        _chk(lib().mgld_rel_bias_grad(_p(drel), _p(plan.index), _p(out), plan.num_buckets, drel.shape[0], 2 * plan.reach + 1, stream_ptr()), what)
+    _vec(what, "drel", drel, (drel.shape[0], 2 * plan.reach + 1), torch.float32)
+    out = _out(what, "out", out, drel, _capturing(), (drel, plan.index), shape=(plan.num_buckets, drel.shape[0]))
+    if not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous")
+    _chk(lib().mgld_rel_bias_grad(_p(drel), _p(plan.index), _p(out), plan.num_buckets, drel.shape[0], 2 * plan.reach + 1, stream_ptr()), what)
     return out
