@@ -43,7 +43,9 @@ constexpr float MA_LOG2E = 1.44269504088896340736f, MA_LN2 = 0.69314718055994530
 #define MA_INF __builtin_inff()
 constexpr int MA_KT = 64;          // keys (rows) per tile
 __host__ __device__ inline int ma_tiles(const int n) { return (n + MA_KT - 1) / MA_KT; }
-constexpr int MA_MAX_REACH = 1024; // a head's distance row lives in LDS
+constexpr int MA_MAX_REACH = 1024; // a head's distance row lives in LDS,
+constexpr int MA_PAD = 64;         // with its end values repeated this often
+__host__ __device__ inline int ma_rel_floats(const int reach) { return 2 * reach + 1 + 2 * MA_PAD; }
 
 // ---- LDS image of a [rows][D] tile: rows of 2 D bytes, 16-byte chunk c of row r at chunk c ^ swz(r).  Two kinds of reads:
 //  * row operand (rows r0 + lane % 32, eight consecutive d): one ds_read_b128, conflict-free (16 rows cover all 64 banks);
@@ -72,6 +74,20 @@ struct Tile {
     return __builtin_bit_cast(V8, r);
   }
 };
+
+// A run of N matrix products whose operands come from LDS: operand i + AHEAD is requested before product i, in this order.  (Left alone the
+// compiler reads each operand right before its product and waits out the LDS latency every time: 2.3 us per 64-key tile at d = 128.)
+template <int N, int AHEAD, typename V8, typename Read, typename Mul>
+__device__ __forceinline__ void ma_stream(const Read read, const Mul mul) {
+  V8 ring[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < N + AHEAD; ++i) {
+    if (i < N) ring[i % (AHEAD + 1)] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+    if (i >= AHEAD) mul(i - AHEAD, ring[(i - AHEAD) % (AHEAD + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 
 // ---- global -> LDS by DMA (`buffer_load_dwordx4 ... lds`: no staging registers, no ds_write pass).  A piece is 1 KiB of the image = 1024 / RB rows;
 // lane l fills slot l of it and therefore fetches chunk (slot ^ swz(row)) of its row.  An offset past the descriptor's end delivers zeros:
@@ -145,7 +161,7 @@ template <int MODE>
 struct Score {
   static constexpr bool CAP = MODE & MA_CAP, SLOPES = MODE & MA_SLOPES, REL = MODE & MA_REL, BIAS = SLOPES || REL;
   float A, B, pre, capA, slope2;
-  const float* rel;          // LDS: the head's distance row in log2 units
+  const float* rel;          // LDS: the head's distance row in log2 units, distance 0 at index reach + MA_PAD
   int reach;
   __device__ Score(const MgldMaskAttn& p, const int h, const float* srel) {
     pre = CAP ? 2.f * MA_LOG2E * p.scale / p.softcap : p.scale * MA_LOG2E;
@@ -153,24 +169,37 @@ struct Score {
     A = BIAS ? 1.f : CAP ? capA : pre;
     B = CAP && !BIAS ? 0.5f * capA : 0.f;
     slope2 = SLOPES ? p.slopes[h] * MA_LOG2E : 0.f;
-    rel = srel;
     reach = p.reach;
+    rel = srel + reach + MA_PAD;
+  }
+  // the bias of a lane's 16 scores of a 32 x 32 block: those at distance delta + off (UP) or delta - off, off = ma_row(0 .. 15) < 32.  The distance
+  // row goes on for MA_PAD entries past both ends, so one clamp of the lane's first distance serves all 16 reads (immediate offsets).
+  struct At { const float* tab; float d; };
+  template <bool UP>
+  __device__ __forceinline__ At at(const int delta) const {
+    At a{nullptr, 0.f};
+    if (SLOPES) a.d = (float)delta;
+    if (REL) a.tab = rel + (UP ? min(max(delta, 1 - MA_PAD - reach), reach + MA_PAD - 32) : min(max(delta, 32 - MA_PAD - reach), reach + MA_PAD - 1) - 31);
+    return a;
   }
   __device__ __forceinline__ float squash(const float acc) const { return -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(acc * pre)); }   // in [-1, 0]
-  __device__ __forceinline__ float biased(const float s2, const int delta) const {      // score in log2 units at distance delta = key - query
-    if (SLOPES) return s2 - slope2 * fabsf((float)delta);
-    if (REL) return s2 + rel[min(max(delta, -reach), reach) + reach];
-    return s2;
+  // score in log2 units from the scaled one
+  template <bool UP>
+  __device__ __forceinline__ float biased(const float f, const float x, const float c, const At a, const int off) const {      // f x + c + bias
+    if (SLOPES) return fmaf(-slope2, fabsf(UP ? a.d + (float)off : a.d - (float)off), CAP ? fmaf(f, x, c) : f * x);
+    if (REL) return CAP ? fmaf(f, x, c + a.tab[UP ? off : 31 - off]) : fmaf(f, x, a.tab[UP ? off : 31 - off]);
+    return 0.f;
   }
-  __device__ __forceinline__ float raw(const float acc, const int delta) const {
+  __device__ __forceinline__ float raw(const float acc, const At a, const int off) const {
     if (!BIAS) return CAP ? squash(acc) : acc;
-    return biased(CAP ? squash(acc) * capA + 0.5f * capA : acc * pre, delta);
+    return biased<true>(CAP ? squash(acc) : acc, CAP ? capA : pre, 0.5f * capA, a, off);
   }
   // P = 2^(score - lse2); sq: the squashed dot product, for the cap's derivative
-  __device__ __forceinline__ float prob(const float acc, const int delta, const float lse2, float& sq) const {
+  template <bool UP>
+  __device__ __forceinline__ float prob(const float acc, const At a, const int off, const float lse2, float& sq) const {
     sq = CAP ? squash(acc) : 0.f;
     if (!BIAS) return __builtin_amdgcn_exp2f(CAP ? sq * capA + (0.5f * capA - lse2) : acc * pre - lse2);
-    return __builtin_amdgcn_exp2f(biased(CAP ? sq * capA + 0.5f * capA : acc * pre, delta) - lse2);
+    return __builtin_amdgcn_exp2f(biased<UP>(CAP ? sq : acc, CAP ? capA : pre, 0.5f * capA, a, off) - lse2);
   }
 };
 
@@ -236,10 +265,13 @@ __device__ __forceinline__ void ma_window(const MgldMaskAttn& p, const RowGroup&
   full = __ballot(a && f);
 }
 
-// the distance row of head h into LDS, in log2 units (all threads of the block; a barrier follows in the caller)
-__device__ __forceinline__ void ma_load_rel(const MgldMaskAttn& p, const int h, float* srel, const float unit) {
-  const int n = 2 * p.reach + 1;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) srel[i] = p.rel[(int64_t)h * n + i] * unit;
+// the distance rows of heads h .. h + n - 1 into LDS, in log2 units (all threads of the block; a barrier follows in the caller)
+__device__ __forceinline__ void ma_load_rel(const MgldMaskAttn& p, const int h, const int n, float* srel) {
+  const int w = ma_rel_floats(p.reach), nr = 2 * p.reach + 1;
+  for (int x = threadIdx.x; x < n * w; x += blockDim.x) {
+    const int g = x / w, e = x - g * w;
+    srel[x] = p.rel[(int64_t)(h + g) * nr + min(max(e - MA_PAD, 0), nr - 1)] * MA_LOG2E;
+  }
 }
 
 // ---- exact row by row, for the few rows whose fast result is not finite: a product with a zero probability turns an infinity or NaN of a

@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
   v8 qf[DK];
 #pragma unroll
   for (int ks = 0; ks < DK; ++ks) qf[ks] = i < p.Nq && ks * 2 + lhi < d8 ? *(const v8*)(Qp + (int64_t)i * p.q_si + ks * 16 + lhi * 8) : zero;
-  if (MODE & MA_REL) ma_load_rel(p, h, srel, MA_LOG2E);
+  if (MODE & MA_REL) ma_load_rel(p, h, 1, srel);
   const Score<MODE> sc(p, h, srel);
   const float thr = 6.f / sc.A;
 
@@ -190,21 +190,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
       const char* const sk = smem + buf * 2 * TBYTES;
       const char* const sv = sk + TBYTES;
       f32x16 st[2];
-#pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        __builtin_amdgcn_sched_barrier(0);
-        st[k2] = ma_zero();
-#pragma unroll
-        for (int ks = 0; ks < DK; ++ks) st[k2] = ma_mfma(TL::template row_frag<v8>(sk, kbase, k2 * 32, ks), qf[ks], st[k2]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      st[0] = ma_zero();
+      st[1] = ma_zero();
+      ma_stream<2 * DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sk, kbase, x / DK * 32, x % DK); },
+                               [&](const int x, const v8 kf) { st[x / DK] = ma_mfma(kf, qf[x % DK], st[x / DK]); });
       const int k0 = t * MA_KT;
       if (MODE) {
-        const int dl = ma_opaque(k0 + 4 * lhi - pos);
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2)
+        for (int k2 = 0; k2 < 2; ++k2) {
+          const auto at = sc.template at<true>(k0 + k2 * 32 + 4 * lhi - pos);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) st[k2][r] = sc.raw(st[k2][r], dl + k2 * 32 + ma_row(r));
+          for (int r = 0; r < 16; ++r) st[k2][r] = sc.raw(st[k2][r], at, ma_row(r));
+        }
       }
       if (!(fl & 2)) {
 #pragma unroll
@@ -214,16 +211,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
         }
       }
       rs.step(st, sc.A, thr);
+      v8 pf[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        __builtin_amdgcn_sched_barrier(0);            // fragment reads stay beside their products (registers)
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = st[s >> 1][(s & 1) * 8 + e];
-        const v8 pf = ma_pack<T>(x);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) rs.o[dt] = ma_mfma(TL::template tr_frag<v8>(sv, vbase, dt, s * 16), pf, rs.o[dt]);
+        pf[s] = ma_pack<T>(x);
       }
+      ma_stream<4 * DT, 4, v8>([&](const int x) { return TL::template tr_frag<v8>(sv, vbase, x % DT, x / DT * 16); },
+                               [&](const int x, const v8 vf) { rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]); });
     }
     buf ^= 1;
     t = tn; fl = fln;
@@ -303,12 +300,9 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     for (int ks = 0; ks < DK; ++ks) qf[ks] = rok && ks * 2 + lhi < d8 ? *(const v8*)(q + ks * 16 + lhi * 8) : zero;
   }
   // a lane's head differs from its neighbour's: the distance rows of the group's heads lie side by side
-  if (MODE & MA_REL) {
-    const int n = 2 * p.reach + 1;
-    for (int e = tid; e < G * n; e += 256) srel[e] = p.rel[(int64_t)hk * G * n + e] * MA_LOG2E;
-  }
+  if (MODE & MA_REL) ma_load_rel(p, hk * G, G, srel);
   __syncthreads();
-  const Score<MODE> sc(p, h, srel + (rok ? r % G : 0) * (2 * p.reach + 1));
+  const Score<MODE> sc(p, h, srel + (rok ? r % G : 0) * ma_rel_floats(p.reach));
   const float thr = 6.f / sc.A;
 
   // this block's tiles: an equal share of those below the rows' limits
@@ -360,29 +354,28 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     __builtin_amdgcn_sched_barrier(0);
     f32x16 st[1];
     st[0] = ma_zero();
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks) st[0] = ma_mfma(TL::template row_frag<v8>(sk, kbase, 0, ks), qf[ks], st[0]);
+    ma_stream<DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sk, kbase, 0, x); }, [&](const int x, const v8 kf) { st[0] = ma_mfma(kf, qf[x], st[0]); });
     const int k0 = t * KH;
     if (MODE) {
-      const int dl = ma_opaque(k0 + 4 * lhi - pos);
+      const auto at = sc.template at<true>(k0 + 4 * lhi - pos);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) st[0][e] = sc.raw(st[0][e], dl + ma_row(e));
+      for (int e = 0; e < 16; ++e) st[0][e] = sc.raw(st[0][e], at, ma_row(e));
     }
     if (!fl) {
       if (docs) ma_mask<true>(st[0], k0, lhi, lim, sdoc + buf * MA_KT, dqm);
       else ma_mask<false>(st[0], k0, lhi, lim, nullptr, 0);
     }
     rs.step(st, sc.A, thr);
+    v8 pf[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      __builtin_amdgcn_sched_barrier(0);
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = st[0][s * 8 + e];
-      const v8 pf = ma_pack<T>(x);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) rs.o[dt] = ma_mfma(TL::template tr_frag<v8>(sv, vbase, dt, s * 16), pf, rs.o[dt]);
+      pf[s] = ma_pack<T>(x);
     }
+    ma_stream<2 * DT, 4, v8>([&](const int x) { return TL::template tr_frag<v8>(sv, vbase, x % DT, x / DT * 16); },
+                             [&](const int x, const v8 vf) { rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]); });
     t = tn; fl = fln; buf ^= 1;
   }
 
@@ -465,12 +458,6 @@ __global__ __launch_bounds__(64) void ma_join_kernel(const MgldMaskAttn p, const
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
-int ma_cus() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-  return n;
-}
-
 struct Plan { bool split; int nsplit, nrb; };
 // few rows: when one block per 128 rows would leave most of the card idle and there are keys to share out
 Plan ma_plan(const MgldMaskAttn* p) {
@@ -479,7 +466,7 @@ Plan ma_plan(const MgldMaskAttn* p) {
   const int64_t rows = (int64_t)G * p->Nq;
   const int64_t blocks = (int64_t)p->batch * p->heads * ((p->Nq + 127) / 128);
   const int64_t packed = (int64_t)p->batch * p->kv_heads * ((rows + 31) / 32);
-  const bool rel_fits = !p->rel || (int64_t)G * (2 * p->reach + 1) * 4 <= 28 * 1024;       // (beside 131 KB of tiles)
+  const bool rel_fits = !p->rel || (int64_t)G * ma_rel_floats(p->reach) * 4 <= 28 * 1024;       // (beside 131 KB of tiles)
   pl.split = rel_fits && (rows + 31) / 32 * p->kv_heads <= 65535 && p->batch <= 65535 && (p->Nq <= 16 || (blocks * 4 <= 256 && nt >= 16));
   if (!pl.split) return pl;
   pl.nrb = (int)((rows + 31) / 32);
@@ -496,7 +483,7 @@ int ma_launch(const MgldMaskAttn& p, hipStream_t st) {
   const Plan pl = ma_plan(&p);
   const i32x4* kdoc = (const i32x4*)p.work;
   float* part = (float*)((char*)p.work + ma_doc_bytes(&p));
-  const int nrel = p.rel ? 2 * p.reach + 1 : 0;
+  const int nrel = p.rel ? ma_rel_floats(p.reach) : 0;
   if (p.doc_q) {
     const int rc = ma_doc_tiles(p, p.work, st);
     if (rc) return rc;
@@ -505,7 +492,7 @@ int ma_launch(const MgldMaskAttn& p, hipStream_t st) {
     const int64_t nqb = (p.Nq + 127) / 128, nb = nqb * p.batch * p.heads;
     MGLD_REQUIRE(nb <= 0x7fffffff, "masked_attention: grid");
     const int lds = 4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + nrel * 4;
-    static_assert(4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + (2 * MA_MAX_REACH + 1) * 4 <= 80 * 1024, "two blocks per CU");
+    static_assert(4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + (2 * MA_MAX_REACH + 1 + 2 * MA_PAD) * 4 <= 80 * 1024, "two blocks per CU");
     if (lds > 64 * 1024) (void)hipFuncSetAttribute((const void*)ma_fwd_kernel<T, D, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     ma_fwd_kernel<T, D, MODE><<<dim3((unsigned)nb), 256, lds, st>>>(p, kdoc, (int)nqb);
     return mgld_check_launch("masked_attention");
@@ -531,7 +518,7 @@ int ma_check(const MgldMaskAttn* p, const bool grad) {
   MGLD_REQUIRE(p->q_pos0 >= -(1 << 30) && p->q_pos0 <= (1 << 30) , "masked_attention: q_pos0");
   MGLD_REQUIRE(!p->rel || (p->reach >= 0 && p->reach <= MA_MAX_REACH), "masked_attention: reach up to 1024");
   MGLD_REQUIRE(!p->rel || !p->slopes, "masked_attention: slopes or rel, not both");
-  MGLD_REQUIRE(!grad || !p->rel || (int64_t)(p->heads / p->kv_heads) * (2 * p->reach + 1) * 4 <= 92 * 1024,
+  MGLD_REQUIRE(!grad || !p->rel || (int64_t)(p->heads / p->kv_heads) * ma_rel_floats(p->reach) * 4 <= 92 * 1024,
                "masked_attention_grad: the distance rows of the query heads that share a key head must fit 92 KB");
   MGLD_REQUIRE(!p->prefix || p->causal, "masked_attention: prefix needs causal");
   MGLD_REQUIRE((p->doc_q != nullptr) == (p->doc_k != nullptr) || p->Nq == 0 || p->Nkv == 0, "masked_attention: doc_q and doc_k go together");

@@ -108,8 +108,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     am = wave_max(am < MA_INF ? am : 0.f);
     if (lane == 0) w.amax[(int64_t)blockIdx.x * 4 + wave] = am;
   }
-  if (MODE & MA_REL) ma_load_rel(p, h, srel, MA_LOG2E);
-  float* const sblk = srel + ((MODE & MA_REL) ? nrel : 0) + wave * (32 * 33 + nrel);
+  if (MODE & MA_REL) ma_load_rel(p, h, 1, srel);
+  float* const sblk = srel + ((MODE & MA_REL) ? ma_rel_floats(p.reach) : 0) + wave * (32 * 33 + nrel);
   float* const sacc = sblk + 32 * 33;
   if (REL)
     for (int e = lane; e < nrel; e += 64) sacc[e] = 0.f;
@@ -147,14 +147,10 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   const int kbase = TL::row_base(lane), tbase = TL::tr_base(lane);
   // a 32-key half of tile t: scores and dP
   auto products = [&](const char* sk, const char* sv, const int k2, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
-    __builtin_amdgcn_sched_barrier(0);
     s = ma_zero();
     dp = ma_zero();
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks) s = ma_mfma(TL::template row_frag<v8>(sk, kbase, k2 * 32, ks), qf[ks], s);
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks) dp = ma_mfma(TL::template row_frag<v8>(sv, kbase, k2 * 32, ks), gf[ks], dp);
-    __builtin_amdgcn_sched_barrier(0);
+    ma_stream<2 * DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(x < DK ? sk : sv, kbase, k2 * 32, x % DK); },
+                             [&](const int x, const v8 f) { if (x < DK) s = ma_mfma(f, qf[x], s); else dp = ma_mfma(f, gf[x - DK], dp); });
   };
   int buf = 0;
   float delta = 0.f;
@@ -174,7 +170,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
           f32x16 s, dp;
           products(sk, sk + TBYTES, k2, s, dp);
           const int k0 = t * MA_KT + k2 * 32;
-          const int dl = ma_opaque(k0 + lhi * 4 - pos), ll = ma_opaque(lim - (k0 + lhi * 4));
+          const auto at = sc.template at<true>(k0 + lhi * 4 - pos);
+        const int ll = ma_opaque(lim - (k0 + lhi * 4));
 #pragma unroll
           for (int rg = 0; rg < 4; ++rg) {
             i32x4 dk4 = {dqm, dqm, dqm, dqm};
@@ -183,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
             for (int e = 0; e < 4; ++e) {
               const int r = rg * 4 + e;
               float sq = 0.f;
-              float x = sc.prob(s[r], dl + rg * 8 + e, lse2, sq) * dp[r];
+              float x = sc.template prob<true>(s[r], at, rg * 8 + e, lse2, sq) * dp[r];
               if (!(fl & 2)) x = (rg * 8 + e < ll) & (dk4[e] == dqm) ? x : 0.f;
               delta += x;
             }
@@ -219,7 +216,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
         f32x16 s, dp;
         products(sk, sv, k2, s, dp);
         const int k0 = t * MA_KT + k2 * 32;
-        const int dl = ma_opaque(k0 + lhi * 4 - pos), ll = ma_opaque(lim - (k0 + lhi * 4));
+        const auto at = sc.template at<true>(k0 + lhi * 4 - pos);
+        const int ll = ma_opaque(lim - (k0 + lhi * 4));
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
           i32x4 dk4 = {dqm, dqm, dqm, dqm};
@@ -228,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
           for (int e = 0; e < 4; ++e) {
             const int r = rg * 4 + e;
             float sq = 0.f;
-            const float pr = sc.prob(s[r], dl + rg * 8 + e, lse2, sq);
+            const float pr = sc.template prob<true>(s[r], at, rg * 8 + e, lse2, sq);
             float ds = pr * (dp[r] - delta);
             if (!(fl & 2)) ds = (rg * 8 + e < ll) & (dk4[e] == dqm) ? ds : 0.f;
             if (REL) dp[r] = ds;                                   // (kept for the diagonals)
@@ -265,16 +263,16 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
             }
           }
         }
+        v8 pf[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          __builtin_amdgcn_sched_barrier(0);
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = s[q * 8 + e];
-          const v8 pf = ma_pack<T>(x);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[dt] = ma_mfma(TL::template tr_frag<v8>(sk, tbase, dt, k2 * 32 + q * 16), pf, o[dt]);
+          pf[q] = ma_pack<T>(x);
         }
+        ma_stream<2 * DT, 3, v8>([&](const int x) { return TL::template tr_frag<v8>(sk, tbase, x % DT, k2 * 32 + x / DT * 16); },
+                                 [&](const int x, const v8 f) { o[x % DT] = ma_mfma(f, pf[x / DT], o[x % DT]); });
       }
     }
     buf ^= 1;
@@ -298,7 +296,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     if (lane == 0) { sacc[0] += far_l; sacc[nrel - 1] += far_r; }
     __syncthreads();
     float* const out = w.rel + ((int64_t)bh * nqb + qb) * nrel;
-    const float* const s0 = srel + nrel + 32 * 33;
+    const float* const s0 = srel + ma_rel_floats(p.reach) + 32 * 33;
     for (int e = tid; e < nrel; e += 256) {
       float f = 0.f;
 #pragma unroll
@@ -327,6 +325,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
   typedef Tile<D> TL;
   constexpr int DK = D / 16, DT = D / 32, ROWS = D == 64 ? 64 : 32, NH = ROWS / 32;
   constexpr bool VLDS = D == 128;
+  constexpr int AHEAD = D == 128 ? 3 : 4;          // operands on their way (at D = 128 a fourth spills)
   constexpr int TBYTES = ROWS * TL::RB, STAT = 3 * MA_KT * 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];      // [2] x {Q, dO}, [2] x {lse, delta, doc numbers} [64], D = 128: V of the block's keys; the distance rows
   char* const sstat = smem + 4 * TBYTES;
@@ -334,8 +333,9 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
   float* const srel = (float*)(sV + (VLDS ? 128 * TL::RB : 0));
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, lhi = lane >> 5;
   const int G = p.heads / p.kv_heads, nbk = p.batch * p.kv_heads;
-  const int per_kb = nbk * nsp;                                     // (the first key blocks have the most rows under a causal mask: they come first)
-  int kb = blockIdx.x / per_kb, rem = blockIdx.x % per_kb;
+  const int per_kb = nbk * nsp;
+  const int kb = blockIdx.x / per_kb;                               // (the first key blocks have the most rows under a causal mask: they come first)
+  int rem = blockIdx.x % per_kb;
   const int split = rem / nbk;
   rem %= nbk;
   const int b = rem / p.kv_heads, hk = rem % p.kv_heads;
@@ -368,10 +368,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
     if constexpr (VLDS) *(v8*)(sV + TL::chunk_at(wave * 32 + l31, ks * 2 + lhi)) = v;        // (read back by this wave only)
     else vf[ks] = v;
   }
-  if (MODE & MA_REL) {
-    const int n = G * (2 * p.reach + 1);
-    for (int e = tid; e < n; e += 256) srel[e] = p.rel[(int64_t)hk * n + e] * MA_LOG2E;
-  }
+  if (MODE & MA_REL) ma_load_rel(p, hk * G, G, srel);
   constexpr bool F16 = __is_same(T, f16);
   const float pup = F16 ? 10.f : 0.f;                                // fp16: P is rounded as 2^10 P, dT as 2^6 g dT
   const float gup = F16 ? ma_pow2_to(w.gmax[0], -5) * 0.0625f : 1.f; // (P carries 2^10 already)
@@ -441,23 +438,21 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
       const char* const sq_ = smem + buf * 2 * TBYTES;
       const char* const sg = sq_ + TBYTES;
       const float* const sl = (const float*)(sstat + buf * STAT);
-      const Score<MODE> sc(p, hk * G + hd, srel + hd * (2 * p.reach + 1));
+      const Score<MODE> sc(p, hk * G + hd, srel + hd * ma_rel_floats(p.reach));
 #pragma unroll
       for (int q2 = 0; q2 < NH; ++q2) {
-        __builtin_amdgcn_sched_barrier(0);
         f32x16 s = ma_zero(), dp = ma_zero();
-#pragma unroll
-        for (int ks = 0; ks < DK; ++ks) s = ma_mfma(TL::template row_frag<v8>(sq_, rbase, q2 * 32, ks), kf[ks], s);
-#pragma unroll
-        for (int ks = 0; ks < DK; ++ks) {
-          v8 v;
-          if constexpr (VLDS) v = TL::template row_frag<v8>(sV, rbase, wave * 32, ks);
-          else v = vf[ks];
-          dp = ma_mfma(TL::template row_frag<v8>(sg, rbase, q2 * 32, ks), v, dp);
+        ma_stream<DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(sq_, rbase, q2 * 32, x); }, [&](const int x, const v8 f) { s = ma_mfma(f, kf[x], s); });
+        if constexpr (VLDS) {
+          v8 vr[2];
+          ma_stream<2 * DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(x & 1 ? sg : sV, rbase, x & 1 ? q2 * 32 : wave * 32, x >> 1); },
+                                   [&](const int x, const v8 f) { if (x & 1) dp = ma_mfma(f, vr[0], dp); else vr[0] = f; });
+        } else {
+          ma_stream<DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sg, rbase, q2 * 32, x); }, [&](const int x, const v8 f) { dp = ma_mfma(f, vf[x], dp); });
         }
-        __builtin_amdgcn_sched_barrier(0);
         const int ib = i0 + q2 * 32;
-        const int dl = ma_opaque(j - (bs.pos0 + ib + lhi * 4)), il = ma_opaque(ib + lhi * 4);
+        const auto at = sc.template at<false>(j - (bs.pos0 + ib + lhi * 4));
+        const int il = ma_opaque(ib + lhi * 4);
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
           const int rr = q2 * 32 + rg * 8 + lhi * 4;
@@ -468,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
           for (int e = 0; e < 4; ++e) {
             const int r = rg * 4 + e;
             float sq = 0.f;
-            float pr = sc.prob(s[r], dl - (rg * 8 + e), lse2[e] - pup, sq);
+            float pr = sc.template prob<false>(s[r], at, rg * 8 + e, lse2[e] - pup, sq);
             float ds = pr * (dp[r] - delta[e]) * gup;
             if (MODE & MA_CAP) ds *= -4.f * sq * (1.f + sq);
             if (!(fl & 2)) {
@@ -481,22 +476,19 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
             dp[r] = ds;
           }
         }
+        v8 pf[4];                                                   // P, then dT
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          __builtin_amdgcn_sched_barrier(0);
+        for (int q = 0; q < 4; ++q) {
           float x[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = s[q * 8 + e];
-          const v8 pf = ma_pack<T>(x);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) ov[dt] = ma_mfma(TL::template tr_frag<v8>(sg, tbase, dt, q2 * 32 + q * 16), pf, ov[dt]);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = dp[q * 8 + e];
-          const v8 df = ma_pack<T>(x);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) ok_[dt] = ma_mfma(TL::template tr_frag<v8>(sq_, tbase, dt, q2 * 32 + q * 16), df, ok_[dt]);
+          for (int e = 0; e < 8; ++e) x[e] = q < 2 ? s[(q & 1) * 8 + e] : dp[(q & 1) * 8 + e];
+          pf[q] = ma_pack<T>(x);
         }
+        ma_stream<4 * DT, AHEAD - 1, v8>([&](const int x) { return TL::template tr_frag<v8>(x < 2 * DT ? sg : sq_, tbase, x % DT, q2 * 32 + (x / DT & 1) * 16); },
+                                 [&](const int x, const v8 f) {
+                                   if (x < 2 * DT) ov[x % DT] = ma_mfma(f, pf[x / DT], ov[x % DT]);
+                                   else ok_[x % DT] = ma_mfma(f, pf[x / DT], ok_[x % DT]);
+                                 });
       }
     }
     buf ^= 1;
@@ -591,7 +583,7 @@ int grad_launch(const MgldMaskAttn& p, hipStream_t st) {
   w.gmax = (float*)(wk + g.gmax);
   w.rel = (float*)(wk + g.rel);
   w.kv = (float*)(wk + g.kv);
-  const int nrel = p.rel ? 2 * p.reach + 1 : 0, G = p.heads / p.kv_heads;
+  const int nrel = p.rel ? 2 * p.reach + 1 : 0, next = p.rel ? ma_rel_floats(p.reach) : 0, G = p.heads / p.kv_heads;
   MGLD_REQUIRE((int64_t)g.nqb * p.batch * p.heads <= 0x7fffffff && (int64_t)g.nkb * p.batch * p.kv_heads * g.nsp <= 0x7fffffff,
                "masked_attention_grad: grid");
   if (p.doc_q) {
@@ -600,7 +592,7 @@ int grad_launch(const MgldMaskAttn& p, hipStream_t st) {
   }
   if (p.Nq > 0) {
     const dim3 grid((unsigned)((int64_t)g.nqb * p.batch * p.heads));
-    const int lds = 4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + nrel * 4;
+    const int lds = 4 * MA_KT * Tile<D>::RB + 2 * MA_KT * 4 + next * 4;
     if constexpr (MODE & MA_REL) {
       if (p.dRel) {
         const int lr = lds + 4 * (32 * 33 + nrel) * 4;
@@ -617,9 +609,10 @@ int grad_launch(const MgldMaskAttn& p, hipStream_t st) {
   if (p.dRel) ma_rel_sum_kernel<<<dim3(cdiv(nrel, 256), p.heads), 256, 0, st>>>(w.rel, p.dRel, p.batch, p.heads, g.nqb, nrel);
   if (p.Nkv > 0) {
     constexpr int ROWS = D == 64 ? 64 : 32;
-    const int lds = 4 * ROWS * Tile<D>::RB + 2 * 3 * MA_KT * 4 + (D == 128 ? 128 * Tile<D>::RB : 0) + G * nrel * 4;
+    const int lds = 4 * ROWS * Tile<D>::RB + 2 * 3 * MA_KT * 4 + (D == 128 ? 128 * Tile<D>::RB : 0) + G * next * 4;
     grad_lds(ma_dkv_kernel<T, D, MODE>, lds);
-    ma_dkv_kernel<T, D, MODE><<<dim3((unsigned)((int64_t)g.nkb * p.batch * p.kv_heads * g.nsp)), 256, lds, st>>>(p, w, g.nkb, g.nsp);
+    const int64_t nb = (int64_t)g.nkb * p.batch * p.kv_heads * g.nsp;
+    ma_dkv_kernel<T, D, MODE><<<dim3((unsigned)nb), 256, lds, st>>>(p, w, g.nkb, g.nsp);
     if (g.nsp > 1) {
       const int64_t n4 = (int64_t)p.batch * p.Nkv * p.kv_heads * 2 * D / 4;
       MGLD_REQUIRE((n4 + 255) / 256 <= 0x7fffffff, "masked_attention_grad: grid");

@@ -6,9 +6,10 @@
 // Bound: HBM (forward 4 bytes per element, gradient 6); everything a head needs sits in the registers of one group of lanes.
 //  * A lane holds P = 8 pairs (two 16-byte loads; P = 4 / 8-byte loads where sizes or alignment ask for it), a head is a group of
 //    d / 2P lanes padded to a power of two, so the sum of squares is log2(group) exchanges and no LDS.
-//  * A group keeps ONE token and walks over heads: the P sines and cosines of its pairs are computed once and stay in registers.
-//    The angle is reduced in fp64 (turns = p * freqs / 2 pi minus its nearest integer: 2^-31 of a turn at p = 2^20, where an fp32 product is
-//    off by 2^-4), then sincospi in fp32.  Each sine is needed by one group per block, so nothing is tabulated.
+//  * The sines of a block's tokens are computed once, one pair per thread, and pass through LDS; a group keeps ONE token and walks over heads with
+//    its P sines and cosines in registers.  (Every group for itself: 96 us on 16384 tokens x 40 heads x 128, the redundant sincospi held
+//    the VALU.)  The angle is reduced in fp64 (turns = p * freqs / 2 pi minus its nearest integer: 2^-31 of a turn at p = 2^20, where an
+//    fp32 product is off by 2^-4), then sincospi in fp32.
 //  * dg is summed in fp32 inside a block (a lane over its tokens and heads, then the groups in order) and in fp64 over the blocks, in a
 //    fixed order: the same call gives the same bits.
 #include "common.h"
@@ -35,19 +36,28 @@ struct PairMap {
   }
 };
 
+template <typename T, int P>
+struct Raw {               // a lane's two vectors as loaded
+  typename qr_vec<T, P>::type u, v;
+};
 template <typename T, int P, bool IL>
-__device__ __forceinline__ void load_pairs(const T* x, const PairMap<P, IL>& m, float (&a)[P], float (&b)[P]) {
-  typedef typename qr_vec<T, P>::type V;
-  const V u = *(const V*)(x + m.e0), v = *(const V*)(x + m.e1);
+__device__ __forceinline__ void fetch(const T* x, const PairMap<P, IL>& m, Raw<T, P>& r) {
+  r.u = *(const typename qr_vec<T, P>::type*)(x + m.e0);
+  r.v = *(const typename qr_vec<T, P>::type*)(x + m.e1);
+}
+template <typename T, int P, bool IL>
+__device__ __forceinline__ void unpack(const Raw<T, P>& r, const bool on, float (&a)[P], float (&b)[P]) {
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     if (IL) {
-      a[i] = (float)(2 * i < P ? u[(2 * i) % P] : v[(2 * i) % P]);
-      b[i] = (float)(2 * i < P ? u[(2 * i + 1) % P] : v[(2 * i + 1) % P]);
+      a[i] = (float)(2 * i < P ? r.u[(2 * i) % P] : r.v[(2 * i) % P]);
+      b[i] = (float)(2 * i < P ? r.u[(2 * i + 1) % P] : r.v[(2 * i + 1) % P]);
     } else {
-      a[i] = (float)u[i];
-      b[i] = (float)v[i];
+      a[i] = (float)r.u[i];
+      b[i] = (float)r.v[i];
     }
+    a[i] = on ? a[i] : 0.f;
+    b[i] = on ? b[i] : 0.f;
   }
 }
 template <typename T, int P, bool IL>
@@ -76,18 +86,28 @@ __device__ __forceinline__ void load_gamma(const float* g, const PairMap<P, IL>&
     b[i] = g && m.on ? g[eb] : 1.f;
   }
 }
+// cosine and sine of the rot_dim / 2 pairs of tokens [row0, row0 + n) -> sc[token][pair]; all 256 threads
+__device__ __forceinline__ void turns_to_lds(const MgldQkRope& p, const int64_t row0, const int n, f32x2* sc) {
+  const int np = p.rot_dim / 2;
+  for (int x = threadIdx.x; x < n * np; x += 256) {
+    const int tok = x / np, j = x - tok * np;
+    const int64_t row = row0 + tok;
+    if (row >= p.rows) break;
+    const double pos = p.pos64 ? (double)((const int64_t*)p.pos)[row] : (double)((const int32_t*)p.pos)[row];
+    double t = pos * (p.freqs[j] * 0.15915494309189533577);
+    t -= rint(t);
+    float s, c;
+    sincospif(2.f * (float)t, &s, &c);
+    sc[x] = f32x2{c, s};
+  }
+}
 template <int P, bool IL>
-__device__ __forceinline__ void turn_of(const MgldQkRope& p, const int64_t row, const PairMap<P, IL>& m, float (&c)[P], float (&s)[P]) {
-  const double pos = p.rot_dim == 0 ? 0. : p.pos64 ? (double)((const int64_t*)p.pos)[row] : (double)((const int32_t*)p.pos)[row];
+__device__ __forceinline__ void lane_turns(const f32x2* sc, const PairMap<P, IL>& m, float (&c)[P], float (&s)[P]) {
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
-    if (m.on && m.rot) {
-      double t = pos * (p.freqs[m.j0 + i] * 0.15915494309189533577);
-      t -= rint(t);
-      sincospif(2.f * (float)t, &s[i], &c[i]);
-    }
+    const f32x2 v = m.on && m.rot ? sc[m.j0 + i] : f32x2{1.f, 0.f};
+    c[i] = v[0];
+    s[i] = v[1];
   }
 }
 template <int LG>
@@ -100,9 +120,9 @@ __device__ __forceinline__ float group_sum(float v) {
 // one block: TB = 256 / (LG * GT) tokens, GT groups per token; a group takes heads h = its index, + GT, ...
 template <typename T, int P, int LG, bool IL>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, const int GT) {
-  const int grp = threadIdx.x / LG, slot = threadIdx.x % LG;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LG / GT) + grp / GT;
-  if (row >= p.rows) return;
+  extern __shared__ __attribute__((aligned(16))) f32x2 sturn[];    // [TB][rot_dim / 2]
+  const int grp = threadIdx.x / LG, slot = threadIdx.x % LG, TB = 256 / LG / GT;
+  const int64_t row0 = (int64_t)blockIdx.x * TB, row = row0 + grp / GT;
   const PairMap<P, IL> m(slot, p.head_dim, p.rot_dim);
   const float inv_d = 1.f / (float)p.head_dim;
   const int first = (int)blockIdx.y * GT + grp % GT, step = GT * (int)gridDim.y, H = p.q.heads + p.k.heads;
@@ -110,19 +130,22 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, c
     return h < p.q.heads ? (const T*)p.q.x + row * p.q.x_sr + (int64_t)h * p.q.x_sh
                          : (const T*)p.k.x + row * p.k.x_sr + (int64_t)(h - p.q.heads) * p.k.x_sh;
   };
-  float c[P], s[P], gqa[P], gqb[P], gka[P], gkb[P], a[P], b[P];
-  if (first < H && m.on) load_pairs<T, P, IL>(src(first), m, a, b);
-  turn_of<P, IL>(p, row, m, c, s);
+  float c[P], s[P], gqa[P], gqb[P], gka[P], gkb[P];
+  Raw<T, P> cur, nxt;
+  if (row < p.rows && first < H && m.on) fetch<T, P, IL>(src(first), m, cur);
+  turns_to_lds(p, row0, TB, sturn);
+  __syncthreads();
+  if (row >= p.rows) return;
+  lane_turns<P, IL>(sturn + (grp / GT) * (p.rot_dim / 2), m, c, s);
   load_gamma<P, IL>(p.q.gamma, m, gqa, gqb);
   load_gamma<P, IL>(p.k.gamma, m, gka, gkb);
   for (int h = first; h < H; h += step) {
-    float na[P], nb[P];
-    if (h + step < H && m.on) load_pairs<T, P, IL>(src(h + step), m, na, nb);      // the next head is on its way while this one is turned
+    if (h + step < H && m.on) fetch<T, P, IL>(src(h + step), m, nxt);               // the next head is on its way while this one is turned
+    float a[P], b[P];
+    unpack<T, P, IL>(cur, m.on, a, b);
     float sq = 0.f;
-    if (m.on) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) sq += a[i] * a[i] + b[i] * b[i];
-    }
+    for (int i = 0; i < P; ++i) sq += a[i] * a[i] + b[i] * b[i];
     const float r = rsqrtf(group_sum<LG>(sq) * inv_d + p.eps);
     const bool isq = h < p.q.heads;
     if (m.on) {
@@ -136,37 +159,47 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, c
       T* y = isq ? (T*)p.q.y + row * p.q.y_sr + (int64_t)h * p.q.y_sh : (T*)p.k.y + row * p.k.y_sr + (int64_t)(h - p.q.heads) * p.k.y_sh;
       store_pairs<T, P, IL>(y, m, ya, yb);
     }
-#pragma unroll
-    for (int i = 0; i < P; ++i) { a[i] = na[i]; b[i] = nb[i]; }
+    cur = nxt;
   }
 }
 
-// gradient: blocks walk over tokens (grid-stride); one side (queries or keys) per blockIdx.y, so a lane sums one gamma gradient
+// gradient: blocks walk over chunks of QR_CHUNK tokens; one side (queries or keys) per blockIdx.y, so a lane sums one gamma gradient.  A group takes
+// (token, head) items in turn, the next one's rows on their way.
+constexpr int QR_CHUNK = 8;
 template <typename T, int P, int LG, bool IL>
-__global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(const MgldQkRope p, const int GT) {
-  extern __shared__ __attribute__((aligned(16))) float sg[];       // [groups][head_dim]
+__global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(const MgldQkRope p) {
+  extern __shared__ __attribute__((aligned(16))) float sg[];       // [QR_CHUNK][rot_dim / 2] turns, later [groups][head_dim] gamma sums
   const MgldHeads& sd = blockIdx.y ? p.k : p.q;
   const int grp = threadIdx.x / LG, slot = threadIdx.x % LG, d = p.head_dim;
   constexpr int NG = 256 / LG;
-  const int TB = NG / GT;
   const PairMap<P, IL> m(slot, d, p.rot_dim);
   const float inv_d = 1.f / (float)d;
+  const int H = (int)sd.heads;
   float ga[P], gb[P], da[P], db[P];
   load_gamma<P, IL>(sd.gamma, m, ga, gb);
 #pragma unroll
   for (int i = 0; i < P; ++i) { da[i] = 0.f; db[i] = 0.f; }
-  for (int64_t row = (int64_t)blockIdx.x * TB + grp / GT; row < p.rows; row += (int64_t)gridDim.x * TB) {
-    float c[P], s[P];
-    turn_of<P, IL>(p, row, m, c, s);
-    for (int h = grp % GT; h < sd.heads; h += GT) {
-      float a[P], b[P], ua[P], ub[P];
-      if (m.on) {
-        load_pairs<T, P, IL>((const T*)sd.x + row * sd.x_sr + (int64_t)h * sd.x_sh, m, a, b);
-        load_pairs<T, P, IL>((const T*)sd.dy + row * sd.dy_sr + (int64_t)h * sd.dy_sh, m, ua, ub);
-      } else {
-#pragma unroll
-        for (int i = 0; i < P; ++i) { a[i] = 0.f; b[i] = 0.f; ua[i] = 0.f; ub[i] = 0.f; }
-      }
+  for (int64_t row0 = (int64_t)blockIdx.x * QR_CHUNK; row0 < p.rows; row0 += (int64_t)gridDim.x * QR_CHUNK) {
+    const int nt = (int)(p.rows - row0 < QR_CHUNK ? p.rows - row0 : QR_CHUNK), items = nt * H;
+    Raw<T, P> cx, cg, nx, ng;
+    auto fetch2 = [&](const int it, Raw<T, P>& x, Raw<T, P>& g) __attribute__((always_inline)) {
+      const int64_t row = row0 + it / H;
+      const int h = it % H;
+      fetch<T, P, IL>((const T*)sd.x + row * sd.x_sr + (int64_t)h * sd.x_sh, m, x);
+      fetch<T, P, IL>((const T*)sd.dy + row * sd.dy_sr + (int64_t)h * sd.dy_sh, m, g);
+    };
+    if (grp < items && m.on) fetch2(grp, cx, cg);
+    __syncthreads();                                               // the previous chunk's turns are used up
+    turns_to_lds(p, row0, nt, (f32x2*)sg);
+    __syncthreads();
+    for (int it = grp; it < items; it += NG) {
+      const int64_t row = row0 + it / H;
+      const int h = it % H;
+      if (it + NG < items && m.on) fetch2(it + NG, nx, ng);
+      float c[P], s[P], a[P], b[P], ua[P], ub[P];
+      unpack<T, P, IL>(cx, m.on, a, b);
+      unpack<T, P, IL>(cg, m.on, ua, ub);
+      lane_turns<P, IL>((const f32x2*)sg + (it / H) * (p.rot_dim / 2), m, c, s);
       float sq = 0.f, dot = 0.f;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
@@ -190,8 +223,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(const MgldQkRope
         }
         store_pairs<T, P, IL>((T*)sd.y + row * sd.y_sr + (int64_t)h * sd.y_sh, m, ya, yb);
       }
+      cx = nx;
+      cg = ng;
     }
   }
+  __syncthreads();
   if (!sd.dgamma) return;
   if (m.on) {
 #pragma unroll
@@ -210,24 +246,26 @@ __global__ __launch_bounds__(256) void qk_norm_rope_grad_kernel(const MgldQkRope
   }
 }
 
-// dgamma[e] = sum over the blocks' partial rows, fp64, fixed order: 16 columns x 16 segments of blocks per block
-__global__ __launch_bounds__(256) void qk_gamma_sum_kernel(const MgldQkRope p, const int nblk) {
-  __shared__ double sd[16][17];
+// dgamma[e] = sum over the blocks' partial rows, fp64, fixed order: 8 columns x 128 segments of blocks per block (a wave reads 8 rows of 32 bytes;
+// 16 columns x 16 segments took 17 us for 1024 rows: one load after the other)
+__global__ __launch_bounds__(1024) void qk_gamma_sum_kernel(const MgldQkRope p, const int nblk) {
+  __shared__ double sd[128][9];
   float* out = blockIdx.y ? p.k.dgamma : p.q.dgamma;
   if (!out) return;
-  const int col = threadIdx.x & 15, seg = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
+  const int col = threadIdx.x & 7, seg = threadIdx.x >> 3, e = blockIdx.x * 8 + col;      // head_dim is a multiple of 8
   double t = 0.;
-  if (e < p.head_dim)
-    for (int i = seg; i < nblk; i += 16) t += (double)p.work[((int64_t)blockIdx.y * nblk + i) * p.head_dim + e];
+#pragma unroll 4
+  for (int i = seg; i < nblk; i += 128) t += (double)p.work[((int64_t)blockIdx.y * nblk + i) * p.head_dim + e];
   sd[seg][col] = t;
   __syncthreads();
-  if (seg == 0 && e < p.head_dim) {
-    for (int i = 1; i < 16; ++i) t += sd[i][col];
-    out[e] = (float)t;
+  for (int o = 64; o > 0; o >>= 1) {
+    if (seg < o) sd[seg][col] += sd[seg + o][col];
+    __syncthreads();
   }
+  if (seg == 0) out[e] = (float)sd[0][col];
 }
 
-constexpr int QR_MAX_BLOCKS = 1024;
+constexpr int QR_MAX_BLOCKS = 1024;       // of the gradient: partial gamma rows
 
 // pairs a lane holds: 8 when sizes and addresses allow 16-byte vectors, else 4, else 0 (refused)
 int qr_pairs(const MgldQkRope* p, const bool grad) {
@@ -261,8 +299,8 @@ int qr_check(const MgldQkRope* p, const bool grad) {
   return MGLD_OK;
 }
 
-int qr_grad_blocks(const int64_t rows, const int TB) {
-  const int64_t n = (rows + TB - 1) / TB;
+int qr_grad_blocks(const int64_t rows) {
+  const int64_t n = (rows + QR_CHUNK - 1) / QR_CHUNK;
   return (int)(n < QR_MAX_BLOCKS ? n : QR_MAX_BLOCKS);
 }
 
@@ -277,16 +315,13 @@ int qr_launch(const MgldQkRope& p, const bool grad, hipStream_t st) {
     else while (GT > 1 && GT / 2 >= H) GT /= 2;
     const int gy = p.rows >= 4096 ? 1 : cdiv(H, GT);
     const int TB = NG / GT;
-    qk_norm_rope_kernel<T, P, LG, IL><<<dim3(cdiv(p.rows, TB), gy), 256, 0, st>>>(p, GT);
+    qk_norm_rope_kernel<T, P, LG, IL><<<dim3(cdiv(p.rows, TB), gy), 256, TB * p.rot_dim * 4, st>>>(p, GT);
     return mgld_check_launch("qk_norm_rope");
   }
-  const int hmax = p.q.heads > p.k.heads ? p.q.heads : p.k.heads;
-  int GT = NG;
-  while (GT > 1 && GT > hmax) GT /= 2;
-  const int nb = qr_grad_blocks(p.rows, NG / GT);
-  const bool gam = p.q.dgamma || p.k.dgamma;
-  qk_norm_rope_grad_kernel<T, P, LG, IL><<<dim3(nb, 2), 256, NG * p.head_dim * 4, st>>>(p, GT);
-  if (gam) qk_gamma_sum_kernel<<<dim3(cdiv(p.head_dim, 16), 2), 256, 0, st>>>(p, nb);
+  const int nb = qr_grad_blocks(p.rows);
+  const int lds = (NG * p.head_dim > QR_CHUNK * p.rot_dim ? NG * p.head_dim : QR_CHUNK * p.rot_dim) * 4;
+  qk_norm_rope_grad_kernel<T, P, LG, IL><<<dim3(nb, 2), 256, lds, st>>>(p);
+  if (p.q.dgamma || p.k.dgamma) qk_gamma_sum_kernel<<<dim3(p.head_dim / 8, 2), 1024, 0, st>>>(p, nb);
   return mgld_check_launch("qk_norm_rope_grad");
 }
 
@@ -318,7 +353,7 @@ extern "C" int mgld_qk_norm_rope(const MgldQkRope* p, void* stream) {
 
 extern "C" int64_t mgld_qk_norm_rope_grad_work(const MgldQkRope* p) {
   if (!p || p->rows <= 0) return 0;
-  return (int64_t)2 * (p->rows < QR_MAX_BLOCKS ? p->rows : QR_MAX_BLOCKS) * p->head_dim * 4;
+  return (int64_t)2 * qr_grad_blocks(p->rows) * p->head_dim * 4;
 }
 
 extern "C" int mgld_qk_norm_rope_grad(const MgldQkRope* p, void* stream) {
@@ -326,7 +361,7 @@ extern "C" int mgld_qk_norm_rope_grad(const MgldQkRope* p, void* stream) {
   if (rc) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (p->rows == 0) {          // no rows: the sums over them are zero
-    if (p->q.dgamma || p->k.dgamma) qk_gamma_sum_kernel<<<dim3(cdiv(p->head_dim, 16), 2), 256, 0, st>>>(*p, 0);
+    if (p->q.dgamma || p->k.dgamma) qk_gamma_sum_kernel<<<dim3(p->head_dim / 8, 2), 1024, 0, st>>>(*p, 0);
     return mgld_check_launch("qk_norm_rope_grad");
   }
   if (p->q.dgamma || p->k.dgamma)
