@@ -48,14 +48,16 @@ constexpr int MA_PAD = 64;         // with its end values repeated this often
 __host__ __device__ inline int ma_rel_floats(const int reach) { return 2 * reach + 1 + 2 * MA_PAD; }
 
 // ---- LDS image of a [rows][D] tile: rows of 2 D bytes, 16-byte chunk c of row r at chunk c ^ swz(r).  Two kinds of reads:
-//  * row operand (rows r0 + lane % 32, eight consecutive d): one ds_read_b128, conflict-free (16 rows cover all 64 banks);
+// The swizzle moves consecutive rows (pairs of them at D = 64) by TWO chunks:
+//  * row operand (rows r0 + lane % 32, eight consecutive d): one ds_read_b128, eight rows in eight different chunks;
 //  * transposed operand (row d = dt * 32 + lane % 32, k = tile rows kb + 4 half + 0..3 and kb + 8 + 4 half + 0..3: the order in which
-//    an accumulator holds its rows): two ds_read_b64_tr_b16, which hand lane i of 16 the four rows of column i of a [4][16] block.
+//    an accumulator holds its rows): two ds_read_b64_tr_b16, which hand lane i of 16 the four rows of column i of a [4][16] block; the
+//    block's four 32-byte pieces lie in different banks (a swizzle by single chunks put two of them into the same ones).
 template <int D>
 struct Tile {
   static constexpr int RB = 2 * D;
   static constexpr int CH = D / 8;                       // 16-byte chunks per row
-  __device__ static __forceinline__ int swz(const int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+  __device__ static __forceinline__ int swz(const int r) { return D == 128 ? (r & 3) << 1 | ((r >> 2) & 1) | (r & 8) : (r & 2) | ((r >> 2) & 1) | (r & 8) >> 1; }
   __device__ static __forceinline__ int chunk_at(const int row, const int c) { return row * RB + ((c ^ swz(row)) << 4); }
   // lane's base for row operands; add (r0 * RB), XOR (ks * 32)
   __device__ static __forceinline__ int row_base(const int lane) { return (lane & 31) * RB + (((lane >> 5) ^ swz(lane & 31)) << 4); }

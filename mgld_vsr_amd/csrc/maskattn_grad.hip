@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   auto products = [&](const char* sk, const char* sv, const int k2, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
     s = ma_zero();
     dp = ma_zero();
-    ma_stream<2 * DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(x < DK ? sk : sv, kbase, k2 * 32, x % DK); },
+    ma_stream<2 * DK, REL && D == 128 ? 3 : 4, v8>([&](const int x) { return TL::template row_frag<v8>(x < DK ? sk : sv, kbase, k2 * 32, x % DK); },
                              [&](const int x, const v8 f) { if (x < DK) s = ma_mfma(f, qf[x], s); else dp = ma_mfma(f, gf[x - DK], dp); });
   };
   int buf = 0;
@@ -220,6 +220,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
         const int ll = ma_opaque(lim - (k0 + lhi * 4));
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
+          if (REL && D == 128) __builtin_amdgcn_sched_barrier(0);
           i32x4 dk4 = {dqm, dqm, dqm, dqm};
           if (docs && !(fl & 2)) dk4 = *(const i32x4*)(sdoc + buf * MA_KT + k2 * 32 + rg * 8 + lhi * 4);
 #pragma unroll
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
           for (int e = 0; e < 8; ++e) x[e] = s[q * 8 + e];
           pf[q] = ma_pack<T>(x);
         }
-        ma_stream<2 * DT, 3, v8>([&](const int x) { return TL::template tr_frag<v8>(sk, tbase, x % DT, k2 * 32 + x / DT * 16); },
+        ma_stream<2 * DT, REL && D == 128 ? 2 : 3, v8>([&](const int x) { return TL::template tr_frag<v8>(sk, tbase, x % DT, k2 * 32 + x / DT * 16); },
                                  [&](const int x, const v8 f) { o[x % DT] = ma_mfma(f, pf[x / DT], o[x % DT]); });
       }
     }
@@ -291,8 +292,12 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
       }
   }
   if (REL) {
-    far_l = wave_sum(far_l);
-    far_r = wave_sum(far_r);
+    const int ln = ma_opaque(lane);                    // (the exchange addresses are made here, not kept through the loops)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      far_l += __int_as_float(__builtin_amdgcn_ds_bpermute((ln ^ o) << 2, __float_as_int(far_l)));
+      far_r += __int_as_float(__builtin_amdgcn_ds_bpermute((ln ^ o) << 2, __float_as_int(far_r)));
+    }
     if (lane == 0) { sacc[0] += far_l; sacc[nrel - 1] += far_r; }
     __syncthreads();
     float* const out = w.rel + ((int64_t)bh * nqb + qb) * nrel;
@@ -325,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
   typedef Tile<D> TL;
   constexpr int DK = D / 16, DT = D / 32, ROWS = D == 64 ? 64 : 32, NH = ROWS / 32;
   constexpr bool VLDS = D == 128;
-  constexpr int AHEAD = D == 128 ? 3 : 4;          // operands on their way (at D = 128 a fourth spills)
+  constexpr int AHEAD = D == 128 ? 3 : 4;          // operands on their way
   constexpr int TBYTES = ROWS * TL::RB, STAT = 3 * MA_KT * 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];      // [2] x {Q, dO}, [2] x {lse, delta, doc numbers} [64], D = 128: V of the block's keys; the distance rows
   char* const sstat = smem + 4 * TBYTES;
@@ -438,23 +443,26 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
       const char* const sq_ = smem + buf * 2 * TBYTES;
       const char* const sg = sq_ + TBYTES;
       const float* const sl = (const float*)(sstat + buf * STAT);
+      const int rb = D == 128 ? ma_opaque(rbase) : rbase, tb = D == 128 ? ma_opaque(tbase) : tbase;      // (registers: the swizzled addresses are made per stage)
       const Score<MODE> sc(p, hk * G + hd, srel + hd * ma_rel_floats(p.reach));
 #pragma unroll
       for (int q2 = 0; q2 < NH; ++q2) {
         f32x16 s = ma_zero(), dp = ma_zero();
-        ma_stream<DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(sq_, rbase, q2 * 32, x); }, [&](const int x, const v8 f) { s = ma_mfma(f, kf[x], s); });
+        ma_stream<DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(sq_, rb, q2 * 32, x); }, [&](const int x, const v8 f) { s = ma_mfma(f, kf[x], s); });
         if constexpr (VLDS) {
           v8 vr[2];
-          ma_stream<2 * DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(x & 1 ? sg : sV, rbase, x & 1 ? q2 * 32 : wave * 32, x >> 1); },
+          ma_stream<2 * DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(x & 1 ? sg : sV, rb, x & 1 ? q2 * 32 : wave * 32, x >> 1); },
                                    [&](const int x, const v8 f) { if (x & 1) dp = ma_mfma(f, vr[0], dp); else vr[0] = f; });
         } else {
-          ma_stream<DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sg, rbase, q2 * 32, x); }, [&](const int x, const v8 f) { dp = ma_mfma(f, vf[x], dp); });
+          ma_stream<DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sg, rb, q2 * 32, x); }, [&](const int x, const v8 f) { dp = ma_mfma(f, vf[x], dp); });
         }
         const int ib = i0 + q2 * 32;
         const auto at = sc.template at<false>(j - (bs.pos0 + ib + lhi * 4));
         const int il = ma_opaque(ib + lhi * 4);
+        v8 pf[4];                                                   // P, then dT
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
+          if (D == 128 && MODE) __builtin_amdgcn_sched_barrier(0);        // (four scores at a time: more in flight spill)
           const int rr = q2 * 32 + rg * 8 + lhi * 4;
           const f32x4 lse2 = *(const f32x4*)(sl + rr) * MA_LOG2E, delta = *(const f32x4*)(sl + 64 + rr);
           i32x4 di = {dj, dj, dj, dj};
@@ -472,19 +480,11 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
               pr = vis ? pr : 0.f;
               ds = vis ? ds : 0.f;
             }
-            s[r] = pr;
-            dp[r] = ds;
+            pf[rg >> 1][(rg & 1) * 4 + e] = (T)pr;                  // rounded to nearest: maskattn.h, ma_pack
+            pf[2 + (rg >> 1)][(rg & 1) * 4 + e] = (T)ds;
           }
         }
-        v8 pf[4];                                                   // P, then dT
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = q < 2 ? s[(q & 1) * 8 + e] : dp[(q & 1) * 8 + e];
-          pf[q] = ma_pack<T>(x);
-        }
-        ma_stream<4 * DT, AHEAD - 1, v8>([&](const int x) { return TL::template tr_frag<v8>(x < 2 * DT ? sg : sq_, tbase, x % DT, q2 * 32 + (x / DT & 1) * 16); },
+        ma_stream<4 * DT, 3, v8>([&](const int x) { return TL::template tr_frag<v8>(x < 2 * DT ? sg : sq_, tb, x % DT, q2 * 32 + (x / DT & 1) * 16); },
                                  [&](const int x, const v8 f) {
                                    if (x < 2 * DT) ov[x % DT] = ma_mfma(f, pf[x / DT], ov[x % DT]);
                                    else ok_[x % DT] = ma_mfma(f, pf[x / DT], ok_[x % DT]);
