@@ -97,30 +97,30 @@ __device__ __forceinline__ void ma_stream(const Read read, const Mul mul) {
 // offset never passes 31 bits however long the tensor.  The instruction is written as asm so that the compiler does not drain the queue in front of
 // the next LDS read; it has no output register, and the kernel waits (ma_dma_wait) before the barrier that hands the tile over.
 #if defined(__HIP_DEVICE_COMPILE__)
-__device__ __forceinline__ void ma_dma16(const unsigned lds, const unsigned voff, const uint64_t base) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)base), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(base >> 32)) & 0xffffu,
-                    0x7fffffffu, 0x00020000u};
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(voff), "s"(rs) : "memory", "m0");
+typedef unsigned ma_rsrc __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ ma_rsrc ma_make_rsrc(const uint64_t a) {
+  return ma_rsrc{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
+}
+// lane l's 16 bytes at base + voff + soff -> LDS bytes lds + 16 l
+__device__ __forceinline__ void ma_dma16(const unsigned lds, const unsigned voff, const ma_rsrc rs, const unsigned soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory", "m0");
 }
 // 64 consecutive 4-byte words (one per lane; words at or past `left` arrive as zeros)
 __device__ __forceinline__ void ma_dma4(const unsigned lds, const int lane, const int left, const void* base) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  const uint64_t a = (uint64_t)base;
-  const u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu,
-                    0x7fffffffu, 0x00020000u};
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
-               "v"(lane < left ? lane * 4u : 0x80000000u), "s"(rs) : "memory", "m0");
+               "v"(lane < left ? lane * 4u : 0x80000000u), "s"(ma_make_rsrc((uint64_t)base)) : "memory", "m0");
 }
 #else
-__device__ __forceinline__ void ma_dma16(const unsigned, const unsigned, const uint64_t) {}
+typedef unsigned ma_rsrc;
+__device__ __forceinline__ ma_rsrc ma_make_rsrc(const uint64_t) { return 0; }
+__device__ __forceinline__ void ma_dma16(const unsigned, const unsigned, const ma_rsrc, const unsigned) {}
 __device__ __forceinline__ void ma_dma4(const unsigned, const int, const int, const void*) {}
 #endif
 __device__ __forceinline__ void ma_dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned ma_lds_addr(const void* s) { return (unsigned)(uintptr_t)(ma_lds)s; }
 
 // ROWS x D tile of one matrix, moved by NW waves: this wave's pieces.  With four waves a wave's pieces lie 16 or 32 rows apart, where the swizzle
-// repeats: one lane offset serves all of them and the base moves.
+// repeats: one lane offset serves all of them and the scalar offset moves.
 template <int D, int ROWS, int NW>
 struct TileDma {
   static constexpr int RPP = 1024 / Tile<D>::RB, NP = ROWS / RPP / NW, STEP = NW * RPP;
@@ -141,7 +141,8 @@ struct TileDma {
   // `left` and, with `ids` (document numbers of the rows), rows without a document arrive as zeros
   __device__ __forceinline__ void load(const void* base, const int64_t first_byte, const int64_t stride, const int left, const unsigned tile,
                                        const int32_t* ids = nullptr) const {
-    const uint64_t a = (uint64_t)base + (uint64_t)first_byte;
+    const ma_rsrc rs = ma_make_rsrc((uint64_t)base + (uint64_t)first_byte);
+    const unsigned to = __builtin_amdgcn_readfirstlane((int)(tile + lds)), step = __builtin_amdgcn_readfirstlane((int)(unsigned)(stride * (2 * STEP)));
     bool ok[NP];
 #pragma unroll
     for (int j = 0; j < NP; ++j) ok[j] = row0 + j * STEP < left;
@@ -150,8 +151,7 @@ struct TileDma {
       for (int j = 0; j < NP; ++j) ok[j] = ok[j] && ids[row0 + j * STEP] >= 0;
     }
 #pragma unroll
-    for (int j = 0; j < NP; ++j)
-      ma_dma16(tile + lds + j * NW * 1024, ok[j] ? voff[SAME ? 0 : j] : 0x80000000u, a + (uint64_t)(stride * (2 * j * STEP)));
+    for (int j = 0; j < NP; ++j) ma_dma16(to + j * NW * 1024, ok[j] ? voff[SAME ? 0 : j] : 0x80000000u, rs, j * step);
   }
 };
 

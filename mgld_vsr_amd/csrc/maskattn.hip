@@ -192,8 +192,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
       f32x16 st[2];
       st[0] = ma_zero();
       st[1] = ma_zero();
-      ma_stream<2 * DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sk, kbase, x / DK * 32, x % DK); },
-                               [&](const int x, const v8 kf) { st[x / DK] = ma_mfma(kf, qf[x % DK], st[x / DK]); });
+      ma_stream<2 * DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sk, kbase, (x & 1) * 32, x >> 1); },
+                               [&](const int x, const v8 kf) { st[x & 1] = ma_mfma(kf, qf[x >> 1], st[x & 1]); });      // two accumulators in turn: no product waits for the one before
       const int k0 = t * MA_KT;
       if (MODE) {
 #pragma unroll
