@@ -79,15 +79,31 @@ struct Tile {
 
 // A run of N matrix products whose operands come from LDS: operand i + AHEAD is requested before product i, in this order.  (Left alone the
 // compiler reads each operand right before its product and waits out the LDS latency every time: 2.3 us per 64-key tile at d = 128.)
+template <int I> struct MaIdx {
+  static constexpr int value = I;
+  constexpr operator int() const { return I; }
+};
+template <int I, int N, int AHEAD, typename V8, typename Read, typename Mul>
+__device__ __forceinline__ void ma_stream_from(V8 (&ring)[AHEAD + 1], const Read& read, const Mul& mul) {
+  if constexpr (I < N + AHEAD) {
+    if constexpr (I < N) ring[I % (AHEAD + 1)] = read(MaIdx<I>{});
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (I >= AHEAD) mul(MaIdx<I - AHEAD>{}, ring[(I - AHEAD) % (AHEAD + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
+    ma_stream_from<I + 1, N, AHEAD, V8>(ring, read, mul);
+  }
+}
 template <int N, int AHEAD, typename V8, typename Read, typename Mul>
 __device__ __forceinline__ void ma_stream(const Read read, const Mul mul) {
   V8 ring[AHEAD + 1];
-#pragma unroll
-  for (int i = 0; i < N + AHEAD; ++i) {
-    if (i < N) ring[i % (AHEAD + 1)] = read(i);
-    __builtin_amdgcn_sched_barrier(0);
-    if (i >= AHEAD) mul(i - AHEAD, ring[(i - AHEAD) % (AHEAD + 1)]);
-    __builtin_amdgcn_sched_barrier(0);
+  ma_stream_from<0, N, AHEAD, V8>(ring, read, mul);
+}
+// f(0), f(1), .. f(N - 1) with constant arguments
+template <int I, int N, typename F>
+__device__ __forceinline__ void ma_each(const F& f) {
+  if constexpr (I < N) {
+    f(MaIdx<I>{});
+    ma_each<I + 1, N>(f);
   }
 }
 
@@ -155,21 +171,18 @@ struct TileDma {
   }
 };
 
-// ---- scores.  A kernel keeps "raw" scores; the score in log2 units is raw * A + B with A > 0, so a softmax probability is one fma and one exp2.
-//  Plain: raw = q.k.   Cap: u = cap tanh(t / cap) = cap (1 - 2 / (1 + e^(2 t / cap))): raw = -1 / (1 + exp2(q.k * pre)), one exp2 and one
-//  reciprocal per score (|error| of u ~ 1e-7 cap).   With a bias: raw is the finished score (A = 1).
+// ---- scores, in log2 units (a probability is one subtraction and one exp2).  Cap: u = cap tanh(t / cap) = cap (1 - 2 / (1 + e^(2 t / cap))):
+//  squash = -1 / (1 + exp2(q.k * pre)), one exp2 and one reciprocal per score (|error| of u ~ 1e-7 cap), u = cap (1 + 2 squash).
 constexpr int MA_CAP = 1, MA_SLOPES = 2, MA_REL = 4;       // MODE bits; slopes and distance rows exclude each other
 template <int MODE>
 struct Score {
   static constexpr bool CAP = MODE & MA_CAP, SLOPES = MODE & MA_SLOPES, REL = MODE & MA_REL, BIAS = SLOPES || REL;
-  float A, B, pre, capA, slope2;
+  float pre, capA, slope2;
   const float* rel;          // LDS: the head's distance row in log2 units, distance 0 at index reach + MA_PAD
   int reach;
   __device__ Score(const MgldMaskAttn& p, const int h, const float* srel) {
     pre = CAP ? 2.f * MA_LOG2E * p.scale / p.softcap : p.scale * MA_LOG2E;
     capA = CAP ? 2.f * MA_LOG2E * p.softcap : 0.f;
-    A = BIAS ? 1.f : CAP ? capA : pre;
-    B = CAP && !BIAS ? 0.5f * capA : 0.f;
     slope2 = SLOPES ? p.slopes[h] * MA_LOG2E : 0.f;
     reach = p.reach;
     rel = srel + reach + MA_PAD;
@@ -192,8 +205,8 @@ struct Score {
     if (REL) return CAP ? fmaf(f, x, c + a.tab[UP ? off : 31 - off]) : fmaf(f, x, a.tab[UP ? off : 31 - off]);
     return 0.f;
   }
-  __device__ __forceinline__ float raw(const float acc, const At a, const int off) const {
-    if (!BIAS) return CAP ? squash(acc) : acc;
+  __device__ __forceinline__ float score(const float acc, const At a, const int off) const {
+    if (!BIAS) return CAP ? fmaf(squash(acc), capA, 0.5f * capA) : acc * pre;
     return biased<true>(CAP ? squash(acc) : acc, CAP ? capA : pre, 0.5f * capA, a, off);
   }
   // P = 2^(score - lse2); sq: the squashed dot product, for the cap's derivative

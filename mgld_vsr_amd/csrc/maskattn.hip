@@ -6,8 +6,8 @@
 //  * Scores are computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16): a lane holds 16 keys of ONE query row per 32-key half tile, so the row
 //    maximum and sum are lane-local plus one exchange with lane ^ 32, and the probabilities are the second product's operand as they lie,
 //    O^T = V^T P^T.  V stays row-major in LDS; its transposed fragments come from ds_read_b64_tr_b16.
-//  * One pass with the running maximum (kept in raw units; it moves only when a tile exceeds it by 2^6, so the accumulator is rarely rescaled:
-//    P <= 2^6 fits fp16) and the sum in fp32.
+//  * One pass with the running maximum (it moves only when a score exceeds it by 2^6, so the accumulator is rarely rescaled: P <= 2^6 fits fp16)
+//    and the sum in fp32.
 //  * Which tiles a block visits, and which of them need no mask, is decided 64 tiles at a time: lane l judges tile t0 + l and two
 //    ballots give the bit masks.  A causal, prefix, length or document mask costs skipped tiles nothing and full tiles nothing.
 #include "maskattn.h"
@@ -32,8 +32,9 @@ __global__ __launch_bounds__(64) void ma_doc_tiles_kernel(const int32_t* dk, con
   }
 }
 
-// one 64-key tile of scores -> probabilities packed for the second product; updates the running maximum, sum and accumulators
-template <typename T, int DT, int NH>
+// a query row's running maximum (log2 units), sum and accumulators
+constexpr float MA_SLACK = 6.f;        // the maximum moves when a score exceeds it by this much: probabilities stay below 2^6
+template <int DT>
 struct RowState {
   f32x16 o[DT];
   float m, l;
@@ -41,17 +42,12 @@ struct RowState {
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = ma_zero();
   }
-  // st: raw scores (masked: -inf); A: log2 units per raw unit; thr: 6 / A.  st becomes the probabilities.
-  __device__ __forceinline__ void step(f32x16 (&st)[NH], const float A, const float thr) {
-    float mx = st[0][0];
-#pragma unroll
-    for (int k2 = 0; k2 < NH; ++k2)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[k2][r]);
+  // the row's new scores reach mx (in this lane's half of the keys)
+  __device__ __forceinline__ void rise(float mx) {
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any(mx > m + thr)) {                       // m = -inf: true as soon as something is visible
-      const float mn = mx > m + thr ? mx : m;
-      const float al = m == -MA_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * A);
+    if (__any(mx > m + MA_SLACK)) {                  // m = -inf: true as soon as something is visible
+      const float mn = mx > m + MA_SLACK ? mx : m;
+      const float al = m == -MA_INF ? 0.f : __builtin_amdgcn_exp2f(m - mn);
       l *= al;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -59,24 +55,13 @@ struct RowState {
         for (int r = 0; r < 16; ++r) o[i][r] *= al;
       m = mn;
     }
-    const float mA = m == -MA_INF ? 0.f : m * A;
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int k2 = 0; k2 < NH; ++k2)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        st[k2][r] = __builtin_amdgcn_exp2f(st[k2][r] * A - mA);
-        st[k2][r + 1] = __builtin_amdgcn_exp2f(st[k2][r + 1] * A - mA);
-        s0 += st[k2][r];
-        s1 += st[k2][r + 1];
-      }
-    l += s0 + s1;
   }
+  __device__ __forceinline__ float base() const { return m == -MA_INF ? 0.f : m; }
 };
 
-// masks a 32-key half of raw scores: keys k0 + ma_row(r) + 4 half at or past `lim`, or of another document than dq
+// masks a 32-key half of the scores: keys k0 + ma_row(r) + 4 half at or past `lim`, or of another document than dq
 template <bool DOCS>
-__device__ __forceinline__ void ma_mask(f32x16& st, const int k0, const int lhi, const int lim, const int* sdoc, const int dq) {
+__device__ __forceinline__ void ma_mask(float* st, const int k0, const int lhi, const int lim, const int* sdoc, const int dq) {
   const int left = ma_opaque(lim - k0 - lhi * 4);
 #pragma unroll
   for (int rg = 0; rg < 4; ++rg) {                     // registers 4 rg .. + 3: four consecutive keys
@@ -92,8 +77,8 @@ __device__ __forceinline__ void ma_mask(f32x16& st, const int k0, const int lhi,
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------------
-// block: 4 waves x 32 query rows of one head; K / V tiles of 64 keys go by DMA into two LDS buffers (tile t + 1 is on its way while tile t
-// feeds the matrix cores), one barrier per tile.
+// block: 4 waves x 32 query rows of one head; K / V tiles of 64 keys go by DMA into two LDS buffers each, K one tile ahead of V, one barrier per
+// tile.  A wave computes the scores of tile t + 1 while it turns those of tile t into probabilities.
 template <typename T, int D, int MODE>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const MgldMaskAttn p, const i32x4* __restrict__ kdoc, const int nqb) {
   typedef typename MaVec<T>::v8 v8;
@@ -143,7 +128,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
   for (int ks = 0; ks < DK; ++ks) qf[ks] = i < p.Nq && ks * 2 + lhi < d8 ? *(const v8*)(Qp + (int64_t)i * p.q_si + ks * 16 + lhi * 8) : zero;
   if (MODE & MA_REL) ma_load_rel(p, h, 1, srel);
   const Score<MODE> sc(p, h, srel);
-  const float thr = 6.f / sc.A;
 
   // tiles to visit
   const int nt = ma_tiles(gb.lim_max);
@@ -164,66 +148,106 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
     return w0 + c;
   };
 
-  // tile t -> buffer `buf`
   const TileDma<D, MA_KT, 4> dk(wave, lane, p.k_si, p.head_dim), dv(wave, lane, p.v_si, p.head_dim);
   const unsigned lds0 = ma_lds_addr(smem);
-  auto load_tile = [&](const int t, const int buf, const int flags) __attribute__((always_inline)) {
+  auto load_k = [&](const int t, const int buf, const int flags) __attribute__((always_inline)) {
     const int k0 = t * MA_KT;
-    const unsigned a = lds0 + buf * 2 * TBYTES;
     const int32_t* const ids = docs ? p.doc_k + b * p.doc_k_sb + k0 : nullptr;
-    dk.load(Kp, (int64_t)k0 * p.k_si * 2, p.k_si, bs.len - k0, a, flags & 4 ? ids : nullptr);
-    dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, bs.len - k0, a + TBYTES, flags & 4 ? ids : nullptr);
+    dk.load(Kp, (int64_t)k0 * p.k_si * 2, p.k_si, bs.len - k0, lds0 + buf * TBYTES, flags & 4 ? ids : nullptr);
     if (docs && wave == 0) ma_dma4(lds0 + 4 * TBYTES + buf * MA_KT * 4, lane, bs.len - k0, ids);      // (zeros past the length: `lim` hides them)
   };
+  auto load_v = [&](const int t, const int buf, const int flags) __attribute__((always_inline)) {
+    const int k0 = t * MA_KT;
+    dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, bs.len - k0, lds0 + (2 + buf) * TBYTES, flags & 4 ? p.doc_k + b * p.doc_k_sb + k0 : nullptr);
+  };
 
-  RowState<T, DT, 2> rs;
+  RowState<DT> rs;
   const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
-  int fl = 0, fln = 0;
-  int t = advance(fl), buf = 0;
-  if (t >= 0) load_tile(t, 0, fl);
+  constexpr int NP = 2 * DK, EPP = 32 / NP;            // products of a 64-key tile (scores, and P V as many), scores per product
+  int fl = 0, fln = 0, buf = 0;
+  int t = advance(fl), tn = -1;
+  float st[32];                                        // tile t's scores
+  float mx;
+  typename Score<MODE>::At at[2];
+  auto places = [&](const int t) __attribute__((always_inline)) {
+    at[0] = sc.template at<true>(t * MA_KT + 4 * lhi - pos);
+    at[1] = sc.template at<true>(t * MA_KT + 32 + 4 * lhi - pos);
+    mx = -MA_INF;
+  };
+  auto finish = [&](auto e_, const f32x16 (&acc)[2]) __attribute__((always_inline)) {
+    constexpr int e = decltype(e_)::value;
+    st[e] = sc.score(acc[e >> 4][e & 15], at[e >> 4], ma_row(e & 15));
+    mx = fmaxf(mx, st[e]);
+  };
+  // masks tile t's scores (document numbers in buffer `buf`) and moves the running maximum
+  auto settle = [&](const int t, const int flags, const int buf) __attribute__((always_inline)) {
+    if (!(flags & 2)) {
+      mx = -MA_INF;
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        if (docs) ma_mask<true>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dqm);
+        else ma_mask<false>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, nullptr, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) mx = fmaxf(mx, st[e]);
+    }
+    rs.rise(mx);
+  };
+  if (t >= 0) {
+    load_k(t, 0, fl);
+    tn = advance(fln);
+    if (tn >= 0) load_k(tn, 1, fln);
+    load_v(t, 0, fl);
+    ma_dma_wait();
+    __syncthreads();
+    f32x16 acc[2] = {ma_zero(), ma_zero()};
+    ma_stream<NP, 4, v8>([&](auto x) { return TL::template row_frag<v8>(smem, kbase, (x & 1) * 32, x >> 1); },
+                         [&](auto x, const v8 kf) { acc[x & 1] = ma_mfma(kf, qf[x >> 1], acc[x & 1]); });
+    places(t);
+    ma_each<0, 32>([&](auto e) __attribute__((always_inline)) { finish(e, acc); });
+    settle(t, fl, 0);
+  }
+  // one tile: its probabilities beside the products of the next tile's scores, then its second product beside the next scores' cap, bias and
+  // maximum.  Each product is followed by the arithmetic of EPP scores, in this order, so that the matrix pipe and the vector pipe work on
+  // one wave at the same time.
   while (t >= 0) {
     ma_dma_wait();
-    __syncthreads();                                   // tile t has landed everywhere, and everyone is done with the other buffer
-    const int tn = advance(fln);
-    if (tn >= 0) load_tile(tn, buf ^ 1, fln);
-    if (fl & 1) {
-      const char* const sk = smem + buf * 2 * TBYTES;
-      const char* const sv = sk + TBYTES;
-      f32x16 st[2];
-      st[0] = ma_zero();
-      st[1] = ma_zero();
-      ma_stream<2 * DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sk, kbase, (x & 1) * 32, x >> 1); },
-                               [&](const int x, const v8 kf) { st[x & 1] = ma_mfma(kf, qf[x >> 1], st[x & 1]); });      // two accumulators in turn: no product waits for the one before
-      const int k0 = t * MA_KT;
-      if (MODE) {
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          const auto at = sc.template at<true>(k0 + k2 * 32 + 4 * lhi - pos);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) st[k2][r] = sc.raw(st[k2][r], at, ma_row(r));
-        }
-      }
-      if (!(fl & 2)) {
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          if (docs) ma_mask<true>(st[k2], k0 + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dqm);
-          else ma_mask<false>(st[k2], k0 + k2 * 32, lhi, lim, nullptr, 0);
-        }
-      }
-      rs.step(st, sc.A, thr);
-      v8 pf[4];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = st[s >> 1][(s & 1) * 8 + e];
-        pf[s] = ma_pack<T>(x);
-      }
-      ma_stream<4 * DT, 4, v8>([&](const int x) { return TL::template tr_frag<v8>(sv, vbase, x % DT, x / DT * 16); },
-                               [&](const int x, const v8 vf) { rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]); });
+    __syncthreads();                                   // the next K and this V have landed everywhere, and everyone is done with the other buffers
+    int flnn = 0, tnn = -1;
+    if (tn >= 0) {
+      load_v(tn, buf ^ 1, fln);
+      tnn = advance(flnn);
+      if (tnn >= 0) load_k(tnn, buf, flnn);
     }
+    const float base = rs.base();
+    v8 pf[4];
+    float l0 = 0.f, l1 = 0.f;
+    auto probs = [&](auto x) __attribute__((always_inline)) {
+      ma_each<0, EPP>([&](auto y) __attribute__((always_inline)) {
+        constexpr int e = decltype(x)::value * EPP + decltype(y)::value;
+        const float pr = __builtin_amdgcn_exp2f(st[e] - base);
+        if (e & 1) l1 += pr; else l0 += pr;
+        pf[e >> 3][e & 7] = (T)pr;                     // rounded to nearest: maskattn.h, ma_pack
+      });
+    };
+    const char* const sk = smem + (buf ^ 1) * TBYTES;
+    const char* const sv = smem + (2 + buf) * TBYTES;
+    const int kb = D == 64 ? ma_opaque(kbase) : kbase, vb = D == 64 ? ma_opaque(vbase) : vbase;      // (D = 64 has 168 registers: the swizzled addresses are made per tile)
+    f32x16 acc[2] = {ma_zero(), ma_zero()};
+    // (after the last tile the scores are those of an old buffer and nobody looks at them: a branch here would move the exponentials in front of it)
+    ma_stream<NP, 4, v8>([&](auto x) { return TL::template row_frag<v8>(sk, kb, (x & 1) * 32, x >> 1); },
+                         [&](auto x, const v8 kf) { acc[x & 1] = ma_mfma(kf, qf[x >> 1], acc[x & 1]); probs(x); });
+    rs.l += l0 + l1;
+    places(tn);
+    ma_stream<NP, 4, v8>([&](auto x) { return TL::template tr_frag<v8>(sv, vb, x % DT, x / DT * 16); },
+                         [&](auto x, const v8 vf) {
+                           rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]);
+                           ma_each<0, EPP>([&](auto y) __attribute__((always_inline)) { finish(MaIdx<decltype(x)::value * EPP + decltype(y)::value>{}, acc); });
+                         });
+    if (tn >= 0) settle(tn, fln, buf ^ 1);
     buf ^= 1;
     t = tn; fl = fln;
+    tn = tnn; fln = flnn;
   }
 
   // ---- epilogue: O[i][d] = O^T[d][i] / l
@@ -237,7 +261,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
   const unsigned long long bz = __ballot(z != z);      // an infinity or NaN came in
   unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
   if (i < p.Nq) {
-    if (p.lse && lhi == 0) p.lse[((int64_t)b * p.heads + h) * p.Nq + i] = l == 0.f ? -MA_INF : (rs.m * sc.A + sc.B + __builtin_amdgcn_logf(l)) * MA_LN2;
+    if (p.lse && lhi == 0) p.lse[((int64_t)b * p.heads + h) * p.Nq + i] = l == 0.f ? -MA_INF : (rs.m + __builtin_amdgcn_logf(l)) * MA_LN2;
     if (!((bad >> l31) & 1)) {
       T* const o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
 #pragma unroll
@@ -303,7 +327,6 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
   if (MODE & MA_REL) ma_load_rel(p, hk * G, G, srel);
   __syncthreads();
   const Score<MODE> sc(p, h, srel + (rok ? r % G : 0) * ma_rel_floats(p.reach));
-  const float thr = 6.f / sc.A;
 
   // this block's tiles: an equal share of those below the rows' limits
   const int nt = ma_tiles(g.lim_max), share = (nt + nsplit - 1) / nsplit;
@@ -338,7 +361,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, g.lim_max - k0, a + TBYTES);
     if (docs) ma_dma4(lds_doc + buf * MA_KT * 4, lane, min(KH, g.lim_max - k0), p.doc_k + b * p.doc_k_sb + k0);
   };
-  RowState<T, DT, 1> rs;
+  RowState<DT> rs;
   const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
   int fl = 0, buf = 0;
   int t = advance(fl);
@@ -352,34 +375,35 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     const char* const sk = smem + wave * 4 * TBYTES + buf * 2 * TBYTES;
     const char* const sv = sk + TBYTES;
     __builtin_amdgcn_sched_barrier(0);
-    f32x16 st[1];
-    st[0] = ma_zero();
-    ma_stream<DK, 4, v8>([&](const int x) { return TL::template row_frag<v8>(sk, kbase, 0, x); }, [&](const int x, const v8 kf) { st[0] = ma_mfma(kf, qf[x], st[0]); });
+    f32x16 acc = ma_zero();
+    ma_stream<DK, 4, v8>([&](auto x) { return TL::template row_frag<v8>(sk, kbase, 0, x); }, [&](auto x, const v8 kf) { acc = ma_mfma(kf, qf[x], acc); });
     const int k0 = t * KH;
-    if (MODE) {
-      const auto at = sc.template at<true>(k0 + 4 * lhi - pos);
+    const auto at = sc.template at<true>(k0 + 4 * lhi - pos);
+    float st[16], mx = -MA_INF;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) st[0][e] = sc.raw(st[0][e], at, ma_row(e));
-    }
+    for (int e = 0; e < 16; ++e) st[e] = sc.score(acc[e], at, ma_row(e));
     if (!fl) {
-      if (docs) ma_mask<true>(st[0], k0, lhi, lim, sdoc + buf * MA_KT, dqm);
-      else ma_mask<false>(st[0], k0, lhi, lim, nullptr, 0);
+      if (docs) ma_mask<true>(st, k0, lhi, lim, sdoc + buf * MA_KT, dqm);
+      else ma_mask<false>(st, k0, lhi, lim, nullptr, 0);
     }
-    rs.step(st, sc.A, thr);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[e]);
+    rs.rise(mx);
+    const float base = rs.base();
     v8 pf[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = st[0][s * 8 + e];
-      pf[s] = ma_pack<T>(x);
+    for (int e = 0; e < 16; ++e) {
+      st[e] = __builtin_amdgcn_exp2f(st[e] - base);
+      rs.l += st[e];
     }
-    ma_stream<2 * DT, 4, v8>([&](const int x) { return TL::template tr_frag<v8>(sv, vbase, x % DT, x / DT * 16); },
-                             [&](const int x, const v8 vf) { rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]); });
+    pf[0] = ma_pack<T>(st);
+    pf[1] = ma_pack<T>(st + 8);
+    ma_stream<2 * DT, 4, v8>([&](auto x) { return TL::template tr_frag<v8>(sv, vbase, x % DT, x / DT * 16); },
+                             [&](auto x, const v8 vf) { rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]); });
     t = tn; fl = fln; buf ^= 1;
   }
 
-  // ---- the four waves' states meet: o * 2^((m_w - M) A)
+  // ---- the four waves' states meet: o * 2^(m_w - M)
   const float l = rs.l + __shfl_xor(rs.l, 32, 64);
   __syncthreads();                                       // every wave is done with its tiles
   if (lhi == 0) { sml[wave * 64 + l31] = rs.m; sml[wave * 64 + 32 + l31] = l; }
@@ -401,7 +425,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float mw = sml[w * 64 + rr];
-      const float f = mw == -MA_INF ? 0.f : __builtin_amdgcn_exp2f((mw - M) * sc.A);
+      const float f = mw == -MA_INF ? 0.f : __builtin_amdgcn_exp2f(mw - M);
       L += sml[w * 64 + 32 + rr] * f;
       const float* ow = (const float*)smem + w * 32 * D + rr * D;
       a0 += ow[lane ^ ((rr & 7) * 4)] * f;
@@ -413,10 +437,10 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
       float* const po = part + slot * (D + 2);
       po[lane] = a0;
       if (D == 128) po[lane + 64] = a1;
-      if (lane == 0) { po[D] = M * sc.A + sc.B; po[D + 1] = L; }           // the maximum in log2 units
+      if (lane == 0) { po[D] = M; po[D + 1] = L; }           // the maximum in log2 units
     } else {
       const bool bad = __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f);
-      if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + hh) * p.Nq + ii] = L == 0.f ? -MA_INF : (M * sc.A + sc.B + __builtin_amdgcn_logf(L)) * MA_LN2;
+      if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + hh) * p.Nq + ii] = L == 0.f ? -MA_INF : (M + __builtin_amdgcn_logf(L)) * MA_LN2;
       if (bad) ma_slow_row<T>(p, b, hh, ii);
       else {
         const float inv = L == 0.f ? 0.f : 1.f / L;

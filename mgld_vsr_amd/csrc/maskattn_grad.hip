@@ -149,8 +149,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   auto products = [&](const char* sk, const char* sv, const int k2, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
     s = ma_zero();
     dp = ma_zero();
-    ma_stream<2 * DK, REL && D == 128 ? 3 : 4, v8>([&](const int x) { return TL::template row_frag<v8>(x & 1 ? sv : sk, kbase, k2 * 32, x >> 1); },
-                             [&](const int x, const v8 f) { if (x & 1) dp = ma_mfma(f, gf[x >> 1], dp); else s = ma_mfma(f, qf[x >> 1], s); });
+    ma_stream<2 * DK, REL && D == 128 ? 3 : 4, v8>([&](auto x) { return TL::template row_frag<v8>(x & 1 ? sv : sk, kbase, k2 * 32, x >> 1); },
+                             [&](auto x, const v8 f) { if (x & 1) dp = ma_mfma(f, gf[x >> 1], dp); else s = ma_mfma(f, qf[x >> 1], s); });
   };
   int buf = 0;
   float delta = 0.f;
@@ -272,8 +272,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
           for (int e = 0; e < 8; ++e) x[e] = s[q * 8 + e];
           pf[q] = ma_pack<T>(x);
         }
-        ma_stream<2 * DT, REL && D == 128 ? 2 : 3, v8>([&](const int x) { return TL::template tr_frag<v8>(sk, tbase, x % DT, k2 * 32 + x / DT * 16); },
-                                 [&](const int x, const v8 f) { o[x % DT] = ma_mfma(f, pf[x / DT], o[x % DT]); });
+        ma_stream<2 * DT, REL && D == 128 ? 2 : 3, v8>([&](auto x) { return TL::template tr_frag<v8>(sk, tbase, x % DT, k2 * 32 + x / DT * 16); },
+                                 [&](auto x, const v8 f) { o[x % DT] = ma_mfma(f, pf[x / DT], o[x % DT]); });
       }
     }
     buf ^= 1;
@@ -450,12 +450,12 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
         f32x16 s = ma_zero(), dp = ma_zero();
         if constexpr (VLDS) {                                       // Q, dO and V fragments in turn
           v8 vr;
-          ma_stream<3 * DK, AHEAD, v8>([&](const int x) { return x % 3 == 0 ? TL::template row_frag<v8>(sq_, rb, q2 * 32, x / 3) : x % 3 == 1 ? TL::template row_frag<v8>(sV, rb, wave * 32, x / 3)
+          ma_stream<3 * DK, AHEAD, v8>([&](auto x) { return x % 3 == 0 ? TL::template row_frag<v8>(sq_, rb, q2 * 32, x / 3) : x % 3 == 1 ? TL::template row_frag<v8>(sV, rb, wave * 32, x / 3)
                                                                                                                                      : TL::template row_frag<v8>(sg, rb, q2 * 32, x / 3); },
-                                       [&](const int x, const v8 f) { if (x % 3 == 0) s = ma_mfma(f, kf[x / 3], s); else if (x % 3 == 1) vr = f; else dp = ma_mfma(f, vr, dp); });
+                                       [&](auto x, const v8 f) { if (x % 3 == 0) s = ma_mfma(f, kf[x / 3], s); else if (x % 3 == 1) vr = f; else dp = ma_mfma(f, vr, dp); });
         } else {
-          ma_stream<2 * DK, AHEAD, v8>([&](const int x) { return TL::template row_frag<v8>(x & 1 ? sg : sq_, rb, q2 * 32, x >> 1); },
-                                       [&](const int x, const v8 f) { if (x & 1) dp = ma_mfma(f, vf[x >> 1], dp); else s = ma_mfma(f, kf[x >> 1], s); });
+          ma_stream<2 * DK, AHEAD, v8>([&](auto x) { return TL::template row_frag<v8>(x & 1 ? sg : sq_, rb, q2 * 32, x >> 1); },
+                                       [&](auto x, const v8 f) { if (x & 1) dp = ma_mfma(f, vf[x >> 1], dp); else s = ma_mfma(f, kf[x >> 1], s); });
         }
         const int ib = i0 + q2 * 32;
         const auto at = sc.template at<false>(j - (bs.pos0 + ib + lhi * 4));
@@ -485,8 +485,8 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
             pf[2 + (rg >> 1)][(rg & 1) * 4 + e] = (T)ds;
           }
         }
-        ma_stream<4 * DT, 3, v8>([&](const int x) { return TL::template tr_frag<v8>(x & 1 ? sq_ : sg, tb, (x >> 1) % DT, q2 * 32 + x / (2 * DT) * 16); },
-                                 [&](const int x, const v8 f) {
+        ma_stream<4 * DT, 3, v8>([&](auto x) { return TL::template tr_frag<v8>(x & 1 ? sq_ : sg, tb, (x >> 1) % DT, q2 * 32 + x / (2 * DT) * 16); },
+                                 [&](auto x, const v8 f) {
                                    if (x & 1) ok_[(x >> 1) % DT] = ma_mfma(f, pf[2 + x / (2 * DT)], ok_[(x >> 1) % DT]);
                                    else ov[(x >> 1) % DT] = ma_mfma(f, pf[x / (2 * DT)], ov[(x >> 1) % DT]);
                                  });
