@@ -117,14 +117,17 @@ typedef unsigned ma_rsrc __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ ma_rsrc ma_make_rsrc(const uint64_t a) {
   return ma_rsrc{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffffu, 0x7fffffffu, 0x00020000u};
 }
-// lane l's 16 bytes at base + voff + soff -> LDS bytes lds + 16 l
+// lane l's 16 bytes at base + voff + soff -> LDS bytes lds + 16 l (lds, base, soff wave-uniform; m0 is put back: the compiler takes it as its own)
 __device__ __forceinline__ void ma_dma16(const unsigned lds, const unsigned voff, const ma_rsrc rs, const unsigned soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory", "m0");
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory");
 }
 // 64 consecutive 4-byte words (one per lane; words at or past `left` arrive as zeros)
 __device__ __forceinline__ void ma_dma4(const unsigned lds, const int lane, const int left, const void* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
-               "v"(lane < left ? lane * 4u : 0x80000000u), "s"(ma_make_rsrc((uint64_t)base)) : "memory", "m0");
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(lane < left ? lane * 4u : 0x80000000u), "s"(ma_make_rsrc((uint64_t)base)) : "memory");
 }
 #else
 typedef unsigned ma_rsrc;
@@ -158,7 +161,7 @@ struct TileDma {
   __device__ __forceinline__ void load(const void* base, const int64_t first_byte, const int64_t stride, const int left, const unsigned tile,
                                        const int32_t* ids = nullptr) const {
     const ma_rsrc rs = ma_make_rsrc((uint64_t)base + (uint64_t)first_byte);
-    const unsigned to = __builtin_amdgcn_readfirstlane((int)(tile + lds)), step = __builtin_amdgcn_readfirstlane((int)(unsigned)(stride * (2 * STEP)));
+    const unsigned step = __builtin_amdgcn_readfirstlane((int)((unsigned)stride * (2 * STEP))), to = __builtin_amdgcn_readfirstlane((int)(tile + lds));
     bool ok[NP];
 #pragma unroll
     for (int j = 0; j < NP; ++j) ok[j] = row0 + j * STEP < left;

@@ -80,7 +80,7 @@ __device__ __forceinline__ void ma_mask(float* st, const int k0, const int lhi, 
 // block: 4 waves x 32 query rows of one head; K / V tiles of 64 keys go by DMA into two LDS buffers each, K one tile ahead of V, one barrier per
 // tile.  A wave computes the scores of tile t + 1 while it turns those of tile t into probabilities.
 template <typename T, int D, int MODE>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const MgldMaskAttn p, const i32x4* __restrict__ kdoc, const int nqb) {
+__global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP) ? 3 : 2) void ma_fwd_kernel(const MgldMaskAttn p, const i32x4* __restrict__ kdoc, const int nqb) {
   typedef typename MaVec<T>::v8 v8;
   typedef Tile<D> TL;
   constexpr int DK = D / 16, DT = D / 32;
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
   RowState<DT> rs;
   const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
   constexpr int NP = 2 * DK, EPP = 32 / NP;            // products of a 64-key tile (scores, and P V as many), scores per product
-  int fl = 0, fln = 0, buf = 0;
+  int fl = 0, fln = 2, buf = 0;
   int t = advance(fl), tn = -1;
   float st[32];                                        // tile t's scores
   float mx;
@@ -179,19 +179,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
     st[e] = sc.score(acc[e >> 4][e & 15], at[e >> 4], ma_row(e & 15));
     mx = fmaxf(mx, st[e]);
   };
-  // masks tile t's scores (document numbers in buffer `buf`) and moves the running maximum
-  auto settle = [&](const int t, const int flags, const int buf) __attribute__((always_inline)) {
-    if (!(flags & 2)) {
-      mx = -MA_INF;
+  // masks tile t's scores (document numbers in buffer `buf`)
+  auto mask = [&](const int t, const int buf) __attribute__((always_inline)) {
+    mx = -MA_INF;
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        if (docs) ma_mask<true>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dqm);
-        else ma_mask<false>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, nullptr, 0);
-      }
-#pragma unroll
-      for (int e = 0; e < 32; ++e) mx = fmaxf(mx, st[e]);
+    for (int k2 = 0; k2 < 2; ++k2) {
+      if (docs) ma_mask<true>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dqm);
+      else ma_mask<false>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, nullptr, 0);
     }
-    rs.rise(mx);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, st[e]);
   };
   if (t >= 0) {
     load_k(t, 0, fl);
@@ -205,7 +202,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
                          [&](auto x, const v8 kf) { acc[x & 1] = ma_mfma(kf, qf[x >> 1], acc[x & 1]); });
     places(t);
     ma_each<0, 32>([&](auto e) __attribute__((always_inline)) { finish(e, acc); });
-    settle(t, fl, 0);
+    if (!(fl & 2)) mask(t, 0);
+    rs.rise(mx);
   }
   // one tile: its probabilities beside the products of the next tile's scores, then its second product beside the next scores' cap, bias and
   // maximum.  Each product is followed by the arithmetic of EPP scores, in this order, so that the matrix pipe and the vector pipe work on
@@ -213,7 +211,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
   while (t >= 0) {
     ma_dma_wait();
     __syncthreads();                                   // the next K and this V have landed everywhere, and everyone is done with the other buffers
-    int flnn = 0, tnn = -1;
+    int flnn = 2, tnn = -1;
     if (tn >= 0) {
       load_v(tn, buf ^ 1, fln);
       tnn = advance(flnn);
@@ -244,7 +242,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void ma_fwd_kernel(const Mgld
                            rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]);
                            ma_each<0, EPP>([&](auto y) __attribute__((always_inline)) { finish(MaIdx<decltype(x)::value * EPP + decltype(y)::value>{}, acc); });
                          });
-    if (tn >= 0) settle(tn, fln, buf ^ 1);
+    if (tn >= 0) {
+      if (!(fln & 2)) mask(tn, buf ^ 1);
+      rs.rise(mx);
+    }
     buf ^= 1;
     t = tn; fl = fln;
     tn = tnn; fln = flnn;
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     }
     const int c = __builtin_ctzll(act);
     act &= act - 1;
-    cur = w0 + c; half = 0; curfull = (int)((full >> c) & 1);
+    cur = __builtin_amdgcn_readfirstlane(w0 + c); half = 0; curfull = (int)((full >> c) & 1);
     fullf = curfull;
     return cur * 2;
   };

@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     const int c = __builtin_ctzll(bact);
     bact &= bact - 1;
     flags = (int)((wact >> c) & 1) | (int)((wfull >> c) & 1) << 1 | (int)((pads >> c) & 1) << 2;
-    return w0 + c;
+    return __builtin_amdgcn_readfirstlane(w0 + c);
   };
   const TileDma<D, MA_KT, 4> dk(wave, lane, p.k_si, p.head_dim), dv(wave, lane, p.v_si, p.head_dim);
   const unsigned lds0 = ma_lds_addr(smem);
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
       const bool mine = turn == split;
       turn = turn + 1 == nsp ? 0 : turn + 1;
       if (!mine) continue;
-      cur = w0 + c; half = 0;
+      cur = __builtin_amdgcn_readfirstlane(w0 + c); half = 0;
       flags = curf = (int)((wact >> c) & 1) | (int)((wfull >> c) & 1) << 1 | (int)((pads >> c) & 1) << 2;
       head = g;
       return cur * MA_KT;
