@@ -128,7 +128,7 @@ def _chk(rc, what):
 
 
 def stream_ptr():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _p(t):
@@ -954,26 +954,31 @@ def _on_its_device(fn):
     def call(*a, **kw):
         for t in (a or kw.values()):
             if t is not None:
+                if isinstance(t, torch.Tensor):
+                    d = t.get_device()
+                    if d >= 0 and d != _current_device():
+                        with torch.cuda.device(d):
+                            return fn(*a, **kw)
                 break
-        else:
-            t = None
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(t.get_device()):
-                return fn(*a, **kw)
         return fn(*a, **kw)
     return call
 
 
+def _current_device():
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else torch.cuda.current_device()
+
+
 def _same_device(what, *ts):
-    _req_cuda(*ts)
     dev = None
     for t in ts:
         if t is not None:
             d = t.get_device()
-            if dev is None:
+            if d != dev:
+                if d < 0:
+                    _req_cuda(t)
+                if dev is not None:
+                    raise ValueError(f"{what}: tensors on different devices")
                 dev = d
-            elif d != dev:
-                raise ValueError(f"{what}: tensors on different devices")
 
 
 class _Memory:
@@ -985,12 +990,18 @@ class _Memory:
                                     "typestr": f"|V{es}", "data": (t.data_ptr(), True)}
 
 
+def _end(t):
+    """one past the tensor's last byte"""
+    if t.is_contiguous():
+        return t.data_ptr() + t.numel() * t.element_size()
+    return t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _overlap(a, b):
     """do two tensors share memory?  Exact for strided views (column blocks of one buffer do not); True where that is too hard to tell"""
     if a is None or b is None or a.numel() == 0 or b.numel() == 0:
         return False
-    ends = [t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
-    if ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr():
+    if _end(a) <= b.data_ptr() or _end(b) <= a.data_ptr():
         return False
     import numpy as np
     try:
@@ -1025,7 +1036,7 @@ def _out(what, name, t, like, capturing, inputs=(), inplace=(), shape=None, dtyp
     if t is None:
         if capturing:
             raise ValueError(f"{what}: pass {name}= while a graph is being captured")
-        return torch.empty_like(like) if shape is None else torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
+        return torch.empty_like(like) if shape is None else like.new_empty(shape, dtype=dtype or like.dtype)
     shape, dtype = tuple(like.shape if shape is None else shape), like.dtype if dtype is None else dtype
     if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == like.device):
         raise ValueError(f"{what}: {name} must be {dtype} {shape} on {like.device}")
@@ -1050,7 +1061,7 @@ def _work(what, work, nbytes, like, capturing, others=()):
     if work is None:
         if capturing:
             raise ValueError(f"{what}: pass work= ({nbytes} bytes) while a graph is being captured")
-        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+        return like.new_empty(nbytes, dtype=torch.uint8)
     if not (work.is_contiguous() and work.device == like.device and work.numel() * work.element_size() >= nbytes and work.data_ptr() % 16 == 0):
         raise ValueError(f"{what}: work must be a contiguous, 16-byte aligned device buffer of at least {nbytes} bytes")
     for t in others:
