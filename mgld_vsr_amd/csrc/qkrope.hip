@@ -3,13 +3,17 @@
 //   n = x r g,  r = (mean_d x^2 + eps)^-1/2;   pair (a, b) of n at position p:  (a cos - b sin, a sin + b cos),  angle = p freqs[j]
 //   gradient: z = R^T dy,  dg = sum_{rows, heads} z x r,  dx = r (g z - x r mean_d(g z x r))
 //
-// Bound: HBM (forward 4 bytes per element, gradient 6); everything a head needs sits in the registers of one group of lanes.
+// Bound: HBM (forward 4 bytes per element, gradient 6; 16384 tokens x 40 heads x 128: 67 us, 5.0 TB/s, and 92 us, 5.5 TB/s, where a
+// large copy reaches 5.1); everything a head needs sits in the registers of one group of lanes.
 //  * A lane holds P = 8 pairs (two 16-byte loads; P = 4 / 8-byte loads where sizes or alignment ask for it), a head is a group of
 //    d / 2P lanes padded to a power of two, so the sum of squares is log2(group) exchanges and no LDS.
 //  * The sines of a block's tokens are computed once, one pair per thread, and pass through LDS; a group keeps ONE token and walks over heads with
 //    its P sines and cosines in registers.  (Every group for itself: 96 us on 16384 tokens x 40 heads x 128, the redundant sincospi held
 //    the VALU.)  The angle is reduced in fp64 (turns = p * freqs / 2 pi minus its nearest integer: 2^-31 of a turn at p = 2^20, where an
 //    fp32 product is off by 2^-4), then sincospi in fp32.
+//  * The gammas lie in LDS (84 vector registers instead of 110: five waves per SIMD, 83 -> 71 us), two heads are in flight per group (-> 70 us),
+//    and the results are stored past the L2 (-> 67 us; a reader right behind it does not lose: 129 -> 122 us with a copy of q following,
+//    25.1 -> 25.4 us where all of it would fit the caches).
 //  * dg is summed in fp32 inside a block (a lane over its tokens and heads, then the groups in order) and in fp64 over the blocks, in a
 //    fixed order: the same call gives the same bits.
 #include "common.h"
@@ -74,8 +78,8 @@ __device__ __forceinline__ void store_pairs(T* y, const PairMap<P, IL>& m, const
       v[i] = (T)b[i];
     }
   }
-  *(V*)(y + m.e0) = u;
-  *(V*)(y + m.e1) = v;
+  __builtin_nontemporal_store(u, (V*)(y + m.e0));
+  __builtin_nontemporal_store(v, (V*)(y + m.e1));
 }
 template <int P, bool IL>
 __device__ __forceinline__ void load_gamma(const float* g, const PairMap<P, IL>& m, float (&a)[P], float (&b)[P]) {
@@ -120,8 +124,9 @@ __device__ __forceinline__ float group_sum(float v) {
 // one block: TB = 256 / (LG * GT) tokens, GT groups per token; a group takes heads h = its index, + GT, ...
 template <typename T, int P, int LG, bool IL>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, const int GT) {
-  extern __shared__ __attribute__((aligned(16))) f32x2 sturn[];    // [TB][rot_dim / 2]
+  extern __shared__ __attribute__((aligned(16))) f32x2 sturn[];    // [TB][rot_dim / 2], then the two gammas
   const int grp = threadIdx.x / LG, slot = threadIdx.x % LG, TB = 256 / LG / GT;
+  float* const sgam = (float*)(sturn + TB * (p.rot_dim / 2));
   const int64_t row0 = (int64_t)blockIdx.x * TB, row = row0 + grp / GT;
   const PairMap<P, IL> m(slot, p.head_dim, p.rot_dim);
   const float inv_d = 1.f / (float)p.head_dim;
@@ -130,17 +135,21 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, c
     return h < p.q.heads ? (const T*)p.q.x + row * p.q.x_sr + (int64_t)h * p.q.x_sh
                          : (const T*)p.k.x + row * p.k.x_sr + (int64_t)(h - p.q.heads) * p.k.x_sh;
   };
-  float c[P], s[P], gqa[P], gqb[P], gka[P], gkb[P];
-  Raw<T, P> cur, nxt;
+  float c[P], s[P];
+  Raw<T, P> cur, nxt, nx2;
   if (row < p.rows && first < H && m.on) fetch<T, P, IL>(src(first), m, cur);
+  if (row < p.rows && first + step < H && m.on) fetch<T, P, IL>(src(first + step), m, nxt);
   turns_to_lds(p, row0, TB, sturn);
+  for (int x = threadIdx.x; x < 2 * p.head_dim; x += 256) {
+    const bool q = x < p.head_dim;
+    const float* g = q ? p.q.gamma : p.k.gamma;
+    sgam[x] = g ? g[q ? x : x - p.head_dim] : 1.f;
+  }
   __syncthreads();
   if (row >= p.rows) return;
   lane_turns<P, IL>(sturn + (grp / GT) * (p.rot_dim / 2), m, c, s);
-  load_gamma<P, IL>(p.q.gamma, m, gqa, gqb);
-  load_gamma<P, IL>(p.k.gamma, m, gka, gkb);
   for (int h = first; h < H; h += step) {
-    if (h + step < H && m.on) fetch<T, P, IL>(src(h + step), m, nxt);               // the next head is on its way while this one is turned
+    if (h + 2 * step < H && m.on) fetch<T, P, IL>(src(h + 2 * step), m, nx2); // two heads are on their way while this one is turned
     float a[P], b[P];
     unpack<T, P, IL>(cur, m.on, a, b);
     float sq = 0.f;
@@ -149,10 +158,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, c
     const float r = rsqrtf(group_sum<LG>(sq) * inv_d + p.eps);
     const bool isq = h < p.q.heads;
     if (m.on) {
-      float ya[P], yb[P];
+      float ya[P], yb[P], ga[P], gb[P];
+      load_gamma<P, IL>(sgam + (isq ? 0 : p.head_dim), m, ga, gb);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const float u = a[i] * r * (isq ? gqa[i] : gka[i]), v = b[i] * r * (isq ? gqb[i] : gkb[i]);
+        const float u = a[i] * r * ga[i], v = b[i] * r * gb[i];
         ya[i] = u * c[i] - v * s[i];
         yb[i] = u * s[i] + v * c[i];
       }
@@ -160,6 +170,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const MgldQkRope p, c
       store_pairs<T, P, IL>(y, m, ya, yb);
     }
     cur = nxt;
+    nxt = nx2;
   }
 }
 
@@ -315,7 +326,7 @@ int qr_launch(const MgldQkRope& p, const bool grad, hipStream_t st) {
     else while (GT > 1 && GT / 2 >= H) GT /= 2;
     const int gy = p.rows >= 4096 ? 1 : cdiv(H, GT);
     const int TB = NG / GT;
-    qk_norm_rope_kernel<T, P, LG, IL><<<dim3(cdiv(p.rows, TB), gy), 256, TB * p.rot_dim * 4, st>>>(p, GT);
+    qk_norm_rope_kernel<T, P, LG, IL><<<dim3(cdiv(p.rows, TB), gy), 256, (TB * p.rot_dim + 2 * p.head_dim) * 4, st>>>(p, GT);
     return mgld_check_launch("qk_norm_rope");
   }
   const int nb = qr_grad_blocks(p.rows);
