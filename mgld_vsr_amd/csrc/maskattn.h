@@ -157,20 +157,24 @@ struct TileDma {
     lds = __builtin_amdgcn_readfirstlane(wave) * 1024;
   }
   // the ROWS rows (stride elements apart) that begin first_byte into the matrix at `base` -> the tile at LDS byte address `tile`; rows at or past
-  // `left` and, with `ids` (document numbers of the rows), rows without a document arrive as zeros
-  __device__ __forceinline__ void load(const void* base, const int64_t first_byte, const int64_t stride, const int left, const unsigned tile,
-                                       const int32_t* ids = nullptr) const {
+  // `left` and rows that gone() names arrive as zeros (gone is asked only if `some`)
+  template <typename Gone>
+  __device__ __forceinline__ void load(const void* base, const int64_t first_byte, const int64_t stride, const int left, const unsigned tile, const bool some,
+                                       const Gone gone) const {
     const ma_rsrc rs = ma_make_rsrc((uint64_t)base + (uint64_t)first_byte);
     const unsigned step = __builtin_amdgcn_readfirstlane((int)((unsigned)stride * (2 * STEP))), to = __builtin_amdgcn_readfirstlane((int)(tile + lds));
     bool ok[NP];
 #pragma unroll
     for (int j = 0; j < NP; ++j) ok[j] = row0 + j * STEP < left;
-    if (ids) {
+    if (some) {
 #pragma unroll
-      for (int j = 0; j < NP; ++j) ok[j] = ok[j] && ids[row0 + j * STEP] >= 0;
+      for (int j = 0; j < NP; ++j) ok[j] = ok[j] && !gone(row0 + j * STEP);
     }
 #pragma unroll
     for (int j = 0; j < NP; ++j) ma_dma16(to + j * NW * 1024, ok[j] ? voff[SAME ? 0 : j] : 0x80000000u, rs, j * step);
+  }
+  __device__ __forceinline__ void load(const void* base, const int64_t first_byte, const int64_t stride, const int left, const unsigned tile) const {
+    load(base, first_byte, stride, left, tile, false, [](int) { return false; });
   }
 };
 

@@ -153,12 +153,13 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   auto load_k = [&](const int t, const int buf, const int flags) __attribute__((always_inline)) {
     const int k0 = t * MA_KT;
     const int32_t* const ids = docs ? p.doc_k + b * p.doc_k_sb + k0 : nullptr;
-    dk.load(Kp, (int64_t)k0 * p.k_si * 2, p.k_si, bs.len - k0, lds0 + buf * TBYTES, flags & 4 ? ids : nullptr);
+    dk.load(Kp, (int64_t)k0 * p.k_si * 2, p.k_si, bs.len - k0, lds0 + buf * TBYTES, flags & 4, [&](const int r) { return ids[r] < 0; });
     if (docs && wave == 0) ma_dma4(lds0 + 4 * TBYTES + buf * MA_KT * 4, lane, bs.len - k0, ids);      // (zeros past the length: `lim` hides them)
   };
   auto load_v = [&](const int t, const int buf, const int flags) __attribute__((always_inline)) {
     const int k0 = t * MA_KT;
-    dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, bs.len - k0, lds0 + (2 + buf) * TBYTES, flags & 4 ? p.doc_k + b * p.doc_k_sb + k0 : nullptr);
+    const int32_t* const ids = docs ? p.doc_k + b * p.doc_k_sb + k0 : nullptr;
+    dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, bs.len - k0, lds0 + (2 + buf) * TBYTES, flags & 4, [&](const int r) { return ids[r] < 0; });
   };
 
   RowState<DT> rs;

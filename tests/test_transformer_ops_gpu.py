@@ -416,6 +416,41 @@ def test_masked_gradient_ignores_padding(hip):
     assert float(dk[0, 64:].abs().max()) == 0 and float(dv[1, 70:].abs().max()) == 0 and float(dq[1, 70:].abs().max()) == 0
 
 
+@pytest.mark.parametrize("what", ["before the first key", "a document without keys", "keys ahead of every query"])
+@pytest.mark.parametrize("dt,d", [(F16, 64), (BF16, 128)])
+def test_masked_gradient_ignores_what_nothing_sees(hip, dt, d, what):
+    """queries that see no key, and keys that no query sees, may hold anything; their gradients are zeros"""
+    g = gen(14)
+    q, k, v, do = (randn(g, 2, 150, 2, d).to(dt) for _ in range(4))
+    kw = dict(causal=True, scale=d ** -0.5, softcap=0.0, q_pos0=0)
+    gone_q, gone_k = torch.zeros(2, 150, dtype=torch.bool), torch.zeros(2, 150, dtype=torch.bool)
+    if what == "before the first key":                       # the queries are the last ones of a shorter sequence
+        kw.update(q_pos0=None, kv_len=torch.tensor([70, 150], dtype=torch.int32))
+        gone_q[0, :80] = True
+        gone_k[0, 70:] = True
+    elif what == "a document without keys":
+        dq = torch.zeros(2, 150, dtype=torch.int32)
+        dk = dq.clone()
+        dq[1, 40:71] = 9
+        kw.update(docs=(dq, dk))
+        gone_q[1, 40:71] = True
+    else:
+        kw.update(q_pos0=-45)
+        gone_q[:, :45] = True
+        gone_k[:, 105:] = True
+    res, tol = reference(q, k, v, do, kw)
+    for x, m in ((q, gone_q), (do, gone_q), (k, gone_k), (v, gone_k)):
+        x[m] = float("nan")
+    c = [x.to(DEV) for x in (q, k, v)]
+    kg = on_gpu(kw)
+    o, lse = hip.masked_attention(*c, **kg)
+    check("o", o, res["o"], tol["o"])
+    dq, dk, dv, _ = hip.masked_attention_grad(*c, o, lse, do.to(DEV), **kg)
+    for n, x in (("dq", dq), ("dk", dk), ("dv", dv)):
+        check(n, x, res[n], tol[n])
+    assert not dq.cpu()[gone_q].any() and not dk.cpu()[gone_k].any() and not dv.cpu()[gone_k].any()
+
+
 @pytest.mark.parametrize("mag", [1e-4, 3e3])
 def test_fp16_gradient_at_other_magnitudes(hip, mag):
     """the gradient of a small or large loss: dS is scaled before its rounding to fp16"""
