@@ -1010,6 +1010,16 @@ def _overlap(a, b):
         return True
 
 
+def _distinct(t):
+    """does every element have a place of its own?  (by nested strides: no for the rare layouts that interleave)"""
+    end = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st < end:
+            return t.numel() == 0
+        end += st * (n - 1)
+    return True
+
+
 def _same_view(a, b):
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
@@ -1040,7 +1050,7 @@ def _out(what, name, t, like, capturing, inputs=(), inplace=(), shape=None, dtyp
     shape, dtype = tuple(like.shape if shape is None else shape), like.dtype if dtype is None else dtype
     if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == like.device):
         raise ValueError(f"{what}: {name} must be {dtype} {shape} on {like.device}")
-    if not (t.numel() == 0 or all(n == 1 or st > 0 for n, st in zip(t.shape, t.stride()))):
+    if not (t.is_contiguous() or _distinct(t)):
         raise ValueError(f"{what}: {name} must not repeat its elements")
     for x in inputs:
         if x is not None and not any(x is y and _same_view(t, y) for y in inplace):

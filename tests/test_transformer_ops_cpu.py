@@ -140,6 +140,7 @@ def test_wrappers_refuse(quiet, monkeypatch):
            dict(rel=f(4, 8)), dict(rel=f(3, 9)), dict(rel=f(4, 2051)), dict(rel=f(4, 9), slopes=f(4)), dict(docs=f(2, 10, dtype=i32)), dict(docs=(f(2, 10), f(2, 20))),
            dict(docs=(f(2, 10, dtype=i32), f(2, 10, dtype=i32))), dict(prefix=f(2, dtype=i32)), dict(prefix=f(3, dtype=i32), causal=True), dict(kv_len=f(2, dtype=torch.int64)),
            dict(kv_len=f(1, dtype=i32)), dict(q_pos0=1 << 31), dict(o=h(2, 10, 4, 32)), dict(o=q), dict(o=h(2, 10, 4, 64).bfloat16()), dict(o=h(2, 1, 4, 64).expand(2, 10, 4, 64)),
+           dict(o=h(4000).as_strided((2, 10, 4, 64), (1000, 64, 32, 1))), dict(o=h(4000).as_strided((2, 10, 4, 64), (640, 256, 64, 1))),
            dict(lse=f(2, 10, 4)), dict(lse=f(2, 4, 10).double()), dict(lse=f(2, 10, 4).transpose(1, 2)),
            dict(q=buf[..., :256].unflatten(2, (4, 64)), o=buf[..., 64:320].unflatten(2, (4, 64)))]
     for b in bad:
