@@ -1325,6 +1325,17 @@ def masked_attention_grad(q, k, v, o, lse, do, *, scale=None, causal=False, soft
     return dq, dk, dv, drel
 
 
+@_on_its_device
+def masked_attention_work_bytes(q, k, v, *, grad=False, scale=None, causal=False, softcap=0.0, slopes=None, rel=None, docs=None, prefix=None, kv_len=None,
+                                q_pos0=None):
+    """bytes of `work` that masked_attention (grad: masked_attention_grad) needs for a call with these options; sizes matter, contents do not"""
+    _, strides, ptr, doc_sb, tail = _mask_attn("masked_attention_work_bytes", q, k, v, scale, causal, softcap, slopes, rel, docs, prefix, kv_len, q_pos0)
+    so, sk, qp = strides[:3], strides[3:6], q.data_ptr()
+    p = MgldMaskAttn(qp, k.data_ptr(), v.data_ptr(), qp, qp, *strides, *so, *ptr, *doc_sb, qp, qp, k.data_ptr(), k.data_ptr(), ptr[1], *so, *so, *sk, *sk,
+                     None, 0, *tail)
+    return int((lib().mgld_masked_attention_grad_work if grad else lib().mgld_masked_attention_work)(C.byref(p)))
+
+
 class RelBuckets:
     """Which bucket each distance -reach .. reach (key - query) belongs to: `index` int32 [2 * reach + 1] on the device."""
 

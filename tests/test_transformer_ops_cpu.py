@@ -273,3 +273,23 @@ def test_oracle_gradient_against_differences():
     pos, fr = torch.tensor([0, 5, 1000]), torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64)
     for il in (False, True):
         assert torch.autograd.gradcheck(lambda a, b: tr.qk_norm_rope(a, pos, fr, b, 1e-6, il), (y, gm))
+
+
+def test_work_sizes(quiet):
+    """the sizes the helper names are the ones the calls ask for"""
+    i32 = torch.int32
+    q, k = h(2, 300, 4, 64), h(2, 300, 2, 64)
+    docs = torch.zeros(2, 300, dtype=i32)
+    rel = torch.zeros(4, 65)
+    for qq, kw in ((q, {}), (q, dict(causal=True, docs=docs)), (q, dict(rel=rel)), (h(2, 2, 4, 64), dict(kv_len=torch.zeros(2, dtype=i32)))):
+        for grad in (False, True):
+            n = hip.masked_attention_work_bytes(qq, k, k, grad=grad, **kw)
+            o, lse = torch.zeros_like(qq), torch.zeros(2, 4, qq.shape[1])
+            run = (lambda w: hip.masked_attention_grad(qq, k, k, o, lse, o.clone(), work=w, **kw)) if grad else (lambda w: hip.masked_attention(qq, k, k, work=w, **kw))
+            if n == 0:
+                continue
+            room = torch.zeros(n + 16, dtype=torch.uint8)
+            room = room[-room.data_ptr() % 16:][:n]
+            run(room)
+            with pytest.raises(ValueError, match=str(n)):
+                run(room[:-1])
