@@ -3,7 +3,7 @@
 //   n = x r g,  r = (mean_d x^2 + eps)^-1/2;   pair (a, b) of n at position p:  (a cos - b sin, a sin + b cos),  angle = p freqs[j]
 //   gradient: z = R^T dy,  dg = sum_{rows, heads} z x r,  dx = r (g z - x r mean_d(g z x r))
 //
-// Bound: HBM (forward 4 bytes per element, gradient 6; 16384 tokens x 40 heads x 128: 67 us, 5.0 TB/s, and 92 us, 5.5 TB/s, where a
+// Bound: HBM (forward 4 bytes per element, gradient 6; 16384 tokens x 40 heads x 128: 67 us, 5.0 TB/s, and 90 us, 5.6 TB/s, where a
 // large copy reaches 5.1); everything a head needs sits in the registers of one group of lanes.
 //  * A lane holds P = 8 pairs (two 16-byte loads; P = 4 / 8-byte loads where sizes or alignment ask for it), a head is a group of
 //    d / 2P lanes padded to a power of two, so the sum of squares is log2(group) exchanges and no LDS.
@@ -276,7 +276,9 @@ __global__ __launch_bounds__(1024) void qk_gamma_sum_kernel(const MgldQkRope p, 
   if (seg == 0) out[e] = (float)sd[0][col];
 }
 
-constexpr int QR_MAX_BLOCKS = 1024;       // of the gradient: partial gamma rows
+// of the gradient, per side (partial gamma rows): four blocks per CU are resident, and every block gets the same number of chunks.  1024 blocks: 95 | 30 us
+// (16384 tokens x 40 heads x 128 | 8195 x 32 x 64), 512 in equal shares: 90 | 26, 2048: 102 | 30; chunks of 4 tokens 98 | 40.
+constexpr int QR_MAX_BLOCKS = 512;
 
 // pairs a lane holds: 8 when sizes and addresses allow 16-byte vectors, else 4, else 0 (refused)
 int qr_pairs(const MgldQkRope* p, const bool grad) {
@@ -311,8 +313,8 @@ int qr_check(const MgldQkRope* p, const bool grad) {
 }
 
 int qr_grad_blocks(const int64_t rows) {
-  const int64_t n = (rows + QR_CHUNK - 1) / QR_CHUNK;
-  return (int)(n < QR_MAX_BLOCKS ? n : QR_MAX_BLOCKS);
+  const int64_t n = (rows + QR_CHUNK - 1) / QR_CHUNK, turns = (n + QR_MAX_BLOCKS - 1) / QR_MAX_BLOCKS;
+  return (int)((n + turns - 1) / turns);
 }
 
 template <typename T, int P, int LG, bool IL>
