@@ -12,8 +12,8 @@
 //  * ma_dkv_kernel, per 128 keys of a key head: S = Q K^T and dP = dO V^T (a lane holds query rows of ONE key), dV^T += dO^T P, dK^T += Q^T dT over
 //    all query heads of the group.  Where that gives too few blocks, the (head, tile) list is dealt to `nsp` blocks whose fp32 sums are added.
 // Bounds and figures: 2 x 2048 tokens, 16 / 4 heads of 128, causal with a prefix: dQ 160 us, dK / dV 146 + 13 us (forward 66).  At d = 128 the LDS reads of 32 rows or keys
-// per wave take as long as the products (wider waves need more registers than there are); causal row blocks differ up to 16-fold in length and 512 of them
-// run in one round, so the longest decide.  With a learned bias (4 x 1024 tokens, 16 heads of 64): dQ 101 us, dK / dV 84 us (forward 40): the diagonals pass through LDS.
+// per wave take as long as the products (wider waves need more registers than there are), and two waves per SIMD hide little of the scores'
+// arithmetic behind them.  With a learned bias (4 x 1024 tokens, 16 heads of 64): dQ 101 us, dK / dV 84 us (forward 40): the diagonals pass through LDS.
 // fp16 operands have 5 exponent bits: dT is scaled by powers of two before its rounding — per row in ma_dq (amax of the row's |dO| to 2^5),
 // by one number for the tensor in ma_dkv (amax of all |dO| to 2^-5) — and P by 2^10 / 2^6 there.  bf16 needs none of it.
 #include "maskattn.h"
