@@ -127,9 +127,8 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
 
   const int i = iw + l31;
   const int pos = bs.pos0 + i;
-  const int lim = i < p.Nq ? bs.limit(p, pos) : 0;
   const int dq = docs && i < p.Nq ? p.doc_q[b * p.doc_q_sb + i] : -1;
-  const int dqm = dq < 0 ? -2 : dq;                    // a row without document equals no key's number
+  const int lim = i < p.Nq && (!docs || dq >= 0) ? bs.limit(p, pos) : 0;         // a row without document sees nothing: its number (any negative one) may be a key's
   v8 qf[DK];
 #pragma unroll
   for (int ks = 0; ks < DK; ++ks) qf[ks] = i < p.Nq && ks * 2 + lhi < d8 ? *(const v8*)(Qp + (int64_t)i * p.q_si + ks * 16 + lhi * 8) : zero;
@@ -192,7 +191,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
     mx = -MA_INF;
 #pragma unroll
     for (int k2 = 0; k2 < 2; ++k2) {
-      if (docs) ma_mask<true>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dqm);
+      if (docs) ma_mask<true>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, sdoc + buf * MA_KT + k2 * 32, dq);
       else ma_mask<false>(st + k2 * 16, t * MA_KT + k2 * 32, lhi, lim, nullptr, 0);
     }
 #pragma unroll
@@ -316,8 +315,8 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
   const int r = rb * 32 + l31;
   const bool rok = r < rows;
   const int i = rok ? r / G : 0, h = hk * G + (rok ? r % G : 0), pos = bs.pos0 + i;
-  const int lim = rok ? bs.limit(p, pos) : 0;
-  const int dq = docs && rok ? p.doc_q[b * p.doc_q_sb + i] : -1, dqm = dq < 0 ? -2 : dq;
+  const int dq = docs && rok ? p.doc_q[b * p.doc_q_sb + i] : -1;
+  const int lim = rok && (!docs || dq >= 0) ? bs.limit(p, pos) : 0;              // (0 where a row has no document)
   const int if_ = rb * 32 / G, il = (min(rb * 32 + 32, rows) - 1) / G;     // queries of this block
   const RowGroup g = ma_row_group(p, bs, b, if_, il - if_ + 1);
   const T* __restrict__ Kp = (const T*)p.K + b * p.k_sb + hk * p.k_sh;
@@ -392,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) st[e] = sc.score(acc[e], at, ma_row(e));
     if (!fl) {
-      if (docs) ma_mask<true>(st, k0, lhi, lim, sdoc + buf * MA_KT, dqm);
+      if (docs) ma_mask<true>(st, k0, lhi, lim, sdoc + buf * MA_KT, dq);
       else ma_mask<false>(st, k0, lhi, lim, nullptr, 0);
     }
 #pragma unroll

@@ -86,8 +86,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   for (int e = 0; e < 8; ++e) zero[e] = (T)0.f;
   const int i = iw + l31, pos = bs.pos0 + i;
   const bool rok = i < p.Nq;
-  const int lim = rok ? bs.limit(p, pos) : 0;
-  const int dq = docs && rok ? p.doc_q[b * p.doc_q_sb + i] : -1, dqm = dq < 0 ? -2 : dq;
+  const int dq = docs && rok ? p.doc_q[b * p.doc_q_sb + i] : -1;
+  const int lim = rok && (!docs || dq >= 0) ? bs.limit(p, pos) : 0;              // (0 where a row has no document)
   const int64_t srow = ((int64_t)b * p.heads + h) * p.Nq + i;
   const float lse = rok ? p.lse[srow] : -MA_INF;
   const float lse2 = lse == -MA_INF ? MA_INF : lse * MA_LOG2E;          // a row that sees nothing: P = 0
@@ -177,14 +177,14 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
         const int ll = ma_opaque(lim - (k0 + lhi * 4));
 #pragma unroll
           for (int rg = 0; rg < 4; ++rg) {
-            i32x4 dk4 = {dqm, dqm, dqm, dqm};
+            i32x4 dk4 = {dq, dq, dq, dq};
             if (docs && !(fl & 2)) dk4 = *(const i32x4*)(sdoc + buf * MA_KT + k2 * 32 + rg * 8 + lhi * 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = rg * 4 + e;
               float sq = 0.f;
               float x = sc.template prob<true>(s[r], at, rg * 8 + e, lse2, sq) * dp[r];
-              if (!(fl & 2)) x = (rg * 8 + e < ll) & (dk4[e] == dqm) ? x : 0.f;
+              if (!(fl & 2)) x = (rg * 8 + e < ll) & (dk4[e] == dq) ? x : 0.f;
               delta += x;
             }
           }
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
           if (REL && D == 128) __builtin_amdgcn_sched_barrier(0);
-          i32x4 dk4 = {dqm, dqm, dqm, dqm};
+          i32x4 dk4 = {dq, dq, dq, dq};
           if (docs && !(fl & 2)) dk4 = *(const i32x4*)(sdoc + buf * MA_KT + k2 * 32 + rg * 8 + lhi * 4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
             float sq = 0.f;
             const float pr = sc.template prob<true>(s[r], at, rg * 8 + e, lse2, sq);
             float ds = pr * (dp[r] - delta);
-            if (!(fl & 2)) ds = (rg * 8 + e < ll) & (dk4[e] == dqm) ? ds : 0.f;
+            if (!(fl & 2)) ds = (rg * 8 + e < ll) & (dk4[e] == dq) ? ds : 0.f;
             if (REL) dp[r] = ds;                                   // (kept for the diagonals)
             if (MODE & MA_CAP) ds *= -4.f * sq * (1.f + sq);       // 1 - tanh^2, tanh = 1 + 2 sq
             s[r] = ds * up;
