@@ -14,13 +14,17 @@
 // Bounds and figures: 2 x 2048 tokens, 16 / 4 heads of 128, causal with a prefix: dQ 160 us, dK / dV 146 + 13 us (forward 66).  At d = 128 the LDS reads of 32 rows or keys
 // per wave take as long as the products (wider waves need more registers than there are), and two waves per SIMD hide little of the scores'
 // arithmetic behind them.  With a learned bias (4 x 1024 tokens, 16 heads of 64): dQ 101 us, dK / dV 84 us (forward 40): the diagonals pass through LDS.
-// fp16 operands have 5 exponent bits: dT is scaled by powers of two before its rounding — per row in ma_dq (amax of the row's |dO| to 2^5),
-// by one number for the tensor in ma_dkv (amax of all |dO| to 2^-5) — and P by 2^10 / 2^6 there.  bf16 needs none of it.
+// fp16 operands have 5 exponent bits: dT is scaled by powers of two before its rounding, per row in ma_dq, by one number for the call in ma_dkv.  The scale
+// comes from dS itself: |dS| = P |dP - D| <= max(P |dP|) + |D|, which the pass for D has at hand (one more maximum per score), so that bound goes to
+// 2^13 .. 2^14 whatever the sizes of dO and V: nothing overflows, and what is rounded to a subnormal lies 2^27 below the largest.  P is rounded as 2^10 P there.
+// bf16 has the exponents and needs none of it.
 #include "maskattn.h"
 
 namespace {
 
-// the largest finite amax -> out[0]
+constexpr int MA_DS_EXP = 13;          // fp16: the largest |dS| a row or a call can have goes to [2^13, 2^14)
+
+// the largest finite bound of |dS| -> out[0]
 __global__ __launch_bounds__(1024) void ma_amax_kernel(const float* amax, const int64_t rows, float* out) {
   __shared__ float sm[16];
   float m = 0.f;
@@ -99,18 +103,6 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     gf[ks] = ok ? *(const v8*)((const T*)p.dO + b * p.do_sb + (int64_t)i * p.do_si + h * p.do_sh + ks * 16 + lhi * 8) : zero;
   }
   constexpr bool F16 = __is_same(T, f16);
-  float up = 1.f;                                                      // fp16: dT is rounded as dT * up
-  if (F16) {
-    float am = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < DK; ++ks)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf((float)gf[ks][e]));
-    am = fmaxf(am, __shfl_xor(am, 32, 64));
-    up = ma_pow2_to(am, 5);
-    am = wave_max(am < MA_INF ? am : 0.f);
-    if (lane == 0) w.amax[(int64_t)blockIdx.x * 4 + wave] = am;
-  }
   if (MODE & MA_REL) ma_load_rel(p, h, 1, srel);
   float* const sblk = srel + ((MODE & MA_REL) ? ma_rel_floats(p.reach) : 0) + wave * (32 * 33 + nrel);
   float* const sacc = sblk + 32 * 33;
@@ -156,8 +148,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
                              [&](auto x, const v8 f) { if (x & 1) dp = ma_mfma(f, gf[x >> 1], dp); else s = ma_mfma(f, qf[x >> 1], s); });
   };
   int buf = 0;
-  float delta = 0.f;
-  {                                                    // D = sum P dP
+  float delta = 0.f, top = 0.f;
+  {                                                    // D = sum P dP; fp16: top = max P |dP|
     int fl = 0, fln = 0;
     int t = advance(fl);
     if (t >= 0) load_tile(t, buf, fl);
@@ -186,6 +178,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
               float x = sc.template prob<true>(s[r], at, rg * 8 + e, lse2, sq) * dp[r];
               if (!(fl & 2)) x = (rg * 8 + e < ll) & (dk4[e] == dq) ? x : 0.f;
               delta += x;
+              if (F16) top = fmaxf(top, fabsf(x));
             }
           }
         }
@@ -195,11 +188,17 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     }
     delta += __shfl_xor(delta, 32, 64);
     if (rok && lhi == 0) w.delta[srow] = delta;
+    if (F16) {
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) + fabsf(delta);
+      const float am = wave_max(top < MA_INF ? top : 0.f);
+      if (lane == 0) w.amax[(int64_t)blockIdx.x * 4 + wave] = am;
+    }
     __syncthreads();                                   // everyone is done with both buffers
     w0 = -64;
     bact = 0;
   }
 
+  const float up = F16 ? ma_pow2_to(top, MA_DS_EXP) : 1.f;             // fp16: dT is rounded as dT * up
   f32x16 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = ma_zero();
@@ -380,8 +379,8 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
   }
   if (MODE & MA_REL) ma_load_rel(p, hk * G, G, srel);
   constexpr bool F16 = __is_same(T, f16);
-  const float pup = F16 ? 10.f : 0.f;                                // fp16: P is rounded as 2^10 P, dT as 2^6 g dT
-  const float gup = F16 ? ma_pow2_to(w.gmax[0], -5) * 0.0625f : 1.f; // (P carries 2^10 already)
+  const float pup = F16 ? 10.f : 0.f;                                // fp16: P is rounded as 2^10 P
+  const float gup = F16 ? ma_pow2_to(w.gmax[0], MA_DS_EXP) * 9.765625e-4f : 1.f;       // (P carries 2^10 already)
 
   // tiles of 64 rows that some key of the block / of the wave is seen from, for every head of the group; dealt to the nsp blocks in turn
   int w0 = -64, g = 0, turn = 0, half = NH == 2 ? 0 : 1, cur = -1, curf = 0;

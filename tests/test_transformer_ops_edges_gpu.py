@@ -66,3 +66,61 @@ def test_padding_rows_of_any_number_hold_anything(hip, Nq, N, pad):
     for n, x in zip(("dq", "dk", "dv"), grads):
         check(n, x, res[n], tol[n])
     assert not o.cpu()[dq < 0].any() and not grads[0].cpu()[dq < 0].any() and not grads[1].cpu()[dk < 0].any()
+
+# ---- fp16 gradients where the values are large ----------------------------------------------------------------------------------------------------
+def check_fp16_grads(hip, q, k, v, do, kw):
+    """reference()'s bounds, with what the smallest step of the scaled dT leaves: a row's (dQ) or the call's (dK) largest |dS| bound, at most
+    2 max|dP|, is brought to 2^13 or more, half a smallest step is 2^-25"""
+    res, tol = reference(q, k, v, do, kw)
+    d, G = q.shape[3], q.shape[2] // k.shape[2]
+    fl = 2 * d * float(do.double().abs().max()) * float(v.double().abs().max()) * 2.0 ** -38
+    keys = k.double().abs().sum(1).repeat_interleave(G, 1)[:, None]
+    rows = q.double().abs().sum(1).unflatten(1, (k.shape[2], G)).sum(2)[:, None]
+    tol["dq"], tol["dk"] = tol["dq"] + kw["scale"] * fl * keys, tol["dk"] + kw["scale"] * fl * rows
+    o, lse, grads = run(hip, q, k, v, do, kw)
+    check("o", o, res["o"], tol["o"])
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        assert not torch.isnan(x).any(), n
+        check(n, x.float().clamp(-65504, 65504), res[n].clamp(-65504, 65504), tol[n])
+    return res
+
+
+@pytest.mark.parametrize("mag,back", [(30.0, 1.0), (1000.0, 1.0), (8000.0, 1e-3), (8000.0, 30.0)])
+@pytest.mark.parametrize("name", ["long", "cap_d64", "d128", "docs", "rel_causal_cap", "tokens"])
+def test_fp16_gradient_of_large_values(hip, name, mag, back):
+    q, k, v, do, kw = problem(name, F16, seed=12)
+    check_fp16_grads(hip, q, k, (v.float() * mag).clamp(-65504, 65504).half(), (do.float() * back).half(), kw)
+
+
+@pytest.mark.parametrize("val,back,chan", [(32.0, 1.0, 128), (40.0, 1.0, 128), (8000.0, 1e-3, 1), (512.0, 1.0, 128), (60000.0, 1.0, 1)])
+def test_fp16_gradient_of_two_keys(hip, val, back, chan):
+    """two keys at P = 1/2 with values +-val in `chan` channels and a constant gradient: dS = +-val back chan / 2, dT is the same; its rounding must not pass
+    fp16's range where dQ = scale dS (k1 - k2) and dK = scale sum dS q stay inside it"""
+    g = gen(43)
+    N = 40
+    q, k = torch.zeros(1, N, 2, 128), torch.zeros(1, 2, 2, 128)
+    q[..., 0], k[..., 0] = 2.0 ** -9 * randn(g, 1, N, 2), 1.0            # the only channel q has is the one the keys share: equal scores
+    k[..., 1:] = 2.0 ** -4 * randn(g, 1, 2, 2, 127)
+    v = torch.zeros(1, 2, 2, 128)
+    v[:, 0, :, :chan], v[:, 1, :, :chan] = val, -val
+    kw = dict(causal=False, scale=128 ** -0.5, softcap=0.0, q_pos0=0)
+    res = check_fp16_grads(hip, q.half(), k.half(), v.half(), torch.full((1, N, 2, 128), back).half(), kw)
+    assert float(res["dq"].abs().max()) < 65504 and float(res["dk"].abs().max()) < 65504
+
+
+def test_fp16_gradient_of_a_quiet_document(hip):
+    """two documents whose losses differ by 2^14: the quiet one's dK and dV keep their bits (bounds of a call of its own, and the smallest step that
+    the loud one leaves)"""
+    q, k, v, do, kw = problem("docs", F16, seed=13)
+    ids = torch.zeros(q.shape[0], q.shape[1], dtype=torch.int32)
+    ids[:, 150:] = 1
+    do[:, 150:] *= 2.0 ** -14
+    kw["docs"] = (ids, ids)
+    check_fp16_grads(hip, q, k, v, do, kw)
+    quiet = [x[:, 150:].contiguous() for x in (q, k, v, do)]
+    alone = dict(kw, docs=None)
+    res, tol = reference(*quiet, {n: x for n, x in alone.items() if x is not None})
+    fl = 2 * q.shape[3] * float(do.double().abs().max()) * float(v.double().abs().max()) * 2.0 ** -38
+    rows = quiet[0].double().abs().sum(1).unflatten(1, (k.shape[2], -1)).sum(2)[:, None]
+    _, _, grads = run(hip, q, k, v, do, kw)
+    check("dk", grads[1][:, 150:], res["dk"], tol["dk"] + kw["scale"] * fl * rows)
