@@ -493,6 +493,7 @@ int mgld_qk_norm_rope_grad(const MgldQkRope* p, void* stream);
 /* Attention with capped scores, distance biases and masks.  For query i of batch row b, standing at position p_i = i + q_pos0 (or, with
  * q_from_end, i + len_b - Nq), and key j < len_b (len_b = kv_len[b] clamped to [0, Nkv], or Nkv):
  *   t = scale q.k;  u = softcap tanh(t / softcap) if softcap > 0, else t;  s = u - slopes[h] |j - p_i| + rel[h][clamp(j - p_i, -reach, reach) + reach]
+ *   (u to 2^-16, or 2^-20 of itself, whatever the cap)
  *   visible: j < len_b, and (causal: j <= p_i or j < prefix[b]), and (documents: doc_q[i] == doc_k[j] >= 0)
  *   o = sum_visible softmax(s) v,  lse = log sum_visible exp(s);   a query that sees nothing: o = 0, lse = -inf, and no gradient.
  * A value or key that a query does not see never reaches that query's result, whatever it holds (infinities, NaN).

@@ -179,17 +179,27 @@ struct TileDma {
 };
 
 // ---- scores, in log2 units (a probability is one subtraction and one exp2).  Cap: u = cap tanh(t / cap) = cap (1 - 2 / (1 + e^(2 t / cap))):
-//  squash = -1 / (1 + exp2(q.k * pre)), one exp2 and one reciprocal per score (|error| of u ~ 1e-7 cap), u = cap (1 + 2 squash).
-constexpr int MA_CAP = 1, MA_SLOPES = 2, MA_REL = 4;       // MODE bits; slopes and distance rows exclude each other
+//  squash = -1 / (1 + exp2(q.k * pre)), one exp2 and one reciprocal per score, u = cap (1 + 2 squash).  That is off by up to 2^-23 of the CAP, whatever the
+//  score: 2^-16 at a cap of 128, and at 1e8 nothing of an ordinary score is left.  Above MA_WIDE_CAP (MODE bit MA_WIDE) scores below a quarter of the cap therefore take
+//  tanh's odd series, u = t (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315 + 62 x^8 / 2835), x = t / cap < 1/4 (the next term is 2^-26), and the others 1 - 2 / (1 + e^2x),
+//  whose error is then 2^-21 of u: relative in both.  It costs nine more instructions per score, so small caps keep the short form: 8192 causal tokens, 32 / 8 heads of
+//  128 bf16, 740 us against 893; 4096 tokens, 16 heads of 64 fp16, 118 against 174; the gradient of 4096 / 2048 such tokens 1042 against 1241, 228 against 279.
+constexpr int MA_CAP = 1, MA_SLOPES = 2, MA_REL = 4, MA_WIDE = 8;       // MODE bits; slopes and distance rows exclude each other; wide: with a cap
+constexpr float MA_WIDE_CAP = 128.f;
+// tanh(x) / x, x^2 = s <= 1/16
+__device__ __forceinline__ float ma_tanh_ratio(const float s) {
+  return fmaf(s, fmaf(s, fmaf(s, fmaf(s, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+}
 template <int MODE>
 struct Score {
-  static constexpr bool CAP = MODE & MA_CAP, SLOPES = MODE & MA_SLOPES, REL = MODE & MA_REL, BIAS = SLOPES || REL;
-  float pre, capA, slope2;
+  static constexpr bool CAP = MODE & MA_CAP, SLOPES = MODE & MA_SLOPES, REL = MODE & MA_REL, WIDE = MODE & MA_WIDE, BIAS = SLOPES || REL;
+  float pre, capA, slope2, scale2;
   const float* rel;          // LDS: the head's distance row in log2 units, distance 0 at index reach + MA_PAD
   int reach;
   __device__ Score(const MgldMaskAttn& p, const int h, const float* srel) {
     pre = CAP ? 2.f * MA_LOG2E * p.scale / p.softcap : p.scale * MA_LOG2E;
-    capA = CAP ? 2.f * MA_LOG2E * p.softcap : 0.f;
+    capA = CAP ? (WIDE ? 1.f : 2.f) * MA_LOG2E * p.softcap : 0.f;
+    scale2 = p.scale * MA_LOG2E;
     slope2 = SLOPES ? p.slopes[h] * MA_LOG2E : 0.f;
     reach = p.reach;
     rel = srel + reach + MA_PAD;
@@ -205,6 +215,21 @@ struct Score {
     return a;
   }
   __device__ __forceinline__ float squash(const float acc) const { return -__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(acc * pre)); }   // in [-1, 0]
+  // wide: u in log2 units, and tanh
+  __device__ __forceinline__ float bend(const float acc, float& th) const {
+    const float a = acc * pre, x = a * (0.5f * MA_LN2), r = ma_tanh_ratio(x * x);
+    const bool near = fabsf(x) < 0.25f;
+    const float far = fmaf(2.f, squash(acc), 1.f);
+    th = near ? x * r : far;
+    return near ? acc * scale2 * r : capA * far;
+  }
+  template <bool UP>
+  __device__ __forceinline__ float raised(const float u, const At a, const int off) const {      // u + bias
+    if (SLOPES) return fmaf(-slope2, fabsf(UP ? a.d + (float)off : a.d - (float)off), u);
+    return REL ? u + a.tab[UP ? off : 31 - off] : u;
+  }
+  // the cap's slope, 1 - tanh^2, from what prob() left
+  __device__ __forceinline__ float slope(const float sq) const { return WIDE ? fmaf(-sq, sq, 1.f) : -4.f * sq * (1.f + sq); }       // (tanh = 1 + 2 squash)
   // score in log2 units from the scaled one
   template <bool UP>
   __device__ __forceinline__ float biased(const float f, const float x, const float c, const At a, const int off) const {      // f x + c + bias
@@ -213,12 +238,21 @@ struct Score {
     return 0.f;
   }
   __device__ __forceinline__ float score(const float acc, const At a, const int off) const {
+    if (WIDE) {
+      float th;
+      const float u = bend(acc, th);
+      return raised<true>(u, a, off);
+    }
     if (!BIAS) return CAP ? fmaf(squash(acc), capA, 0.5f * capA) : acc * pre;
     return biased<true>(CAP ? squash(acc) : acc, CAP ? capA : pre, 0.5f * capA, a, off);
   }
-  // P = 2^(score - lse2); sq: the squashed dot product, for the cap's derivative
+  // P = 2^(score - lse2); sq: the squashed dot product (wide: tanh), for slope()
   template <bool UP>
   __device__ __forceinline__ float prob(const float acc, const At a, const int off, const float lse2, float& sq) const {
+    if (WIDE) {
+      const float u = bend(acc, sq);
+      return __builtin_amdgcn_exp2f(raised<UP>(u, a, off) - lse2);
+    }
     sq = CAP ? squash(acc) : 0.f;
     if (!BIAS) return __builtin_amdgcn_exp2f(CAP ? sq * capA + (0.5f * capA - lse2) : acc * pre - lse2);
     return __builtin_amdgcn_exp2f(biased<UP>(CAP ? sq : acc, CAP ? capA : pre, 0.5f * capA, a, off) - lse2);
@@ -315,7 +349,10 @@ __device__ __forceinline__ void ma_slow_row(const MgldMaskAttn& p, const int b, 
     float t = 0.f;
     for (int e = 0; e < d; ++e) t += (float)q[e] * (float)k[e];
     t *= p.scale;
-    if (cap) t = p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * (2.f * MA_LOG2E / p.softcap))));
+    if (cap) {
+      const float x = t / p.softcap;
+      t = fabsf(x) < 0.25f ? t * ma_tanh_ratio(x * x) : p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * MA_LOG2E))));
+    }
     const int delta = j - pos;
     if (p.slopes) t -= p.slopes[h] * fabsf((float)delta);
     if (p.rel) t += p.rel[(int64_t)h * (2 * p.reach + 1) + min(max(delta, -p.reach), p.reach) + p.reach];
@@ -357,7 +394,7 @@ inline int64_t ma_doc_bytes(const MgldMaskAttn* p) {
 
 }  // namespace
 
-inline int ma_mode(const MgldMaskAttn* p) { return (p->softcap > 0.f ? MA_CAP : 0) | (p->slopes ? MA_SLOPES : 0) | (p->rel ? MA_REL : 0); }
+inline int ma_mode(const MgldMaskAttn* p) { return (p->softcap > 0.f ? MA_CAP : 0) | (p->softcap > MA_WIDE_CAP ? MA_WIDE : 0) | (p->slopes ? MA_SLOPES : 0) | (p->rel ? MA_REL : 0); }
 // calls launch<T, D, MODE>(p, st) for the problem's type, head size and score form
 #define MA_DISPATCH_MODE(launch, T, D, p, st)                                        \
   switch (ma_mode(p)) {                                                              \
@@ -366,7 +403,10 @@ inline int ma_mode(const MgldMaskAttn* p) { return (p->softcap > 0.f ? MA_CAP : 
     case MA_SLOPES: return launch<T, D, MA_SLOPES>(*p, st);                          \
     case MA_SLOPES | MA_CAP: return launch<T, D, MA_SLOPES | MA_CAP>(*p, st);        \
     case MA_REL: return launch<T, D, MA_REL>(*p, st);                                \
-    default: return launch<T, D, MA_REL | MA_CAP>(*p, st);                           \
+    case MA_REL | MA_CAP: return launch<T, D, MA_REL | MA_CAP>(*p, st);              \
+    case MA_WIDE | MA_CAP: return launch<T, D, MA_WIDE | MA_CAP>(*p, st);            \
+    case MA_WIDE | MA_SLOPES | MA_CAP: return launch<T, D, MA_WIDE | MA_SLOPES | MA_CAP>(*p, st); \
+    default: return launch<T, D, MA_WIDE | MA_REL | MA_CAP>(*p, st);                 \
   }
 #define MA_DISPATCH(launch, p, st)                                                   \
   if (p->bf16) {                                                                     \

@@ -171,6 +171,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   RowState<DT> rs;
   const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
   constexpr int NP = 2 * DK, EPP = 32 / NP;            // products of a 64-key tile (scores, and P V as many), scores per product
+  constexpr bool LATE = D == 128 && (MODE & MA_WIDE) && (MODE & (MA_REL | MA_SLOPES));       // the next scores after the second product, not beside it (registers)
   int fl = 0, fln = 2, buf = 0;
   int t = advance(fl), tn = -1;
   float st[32];                                        // tile t's scores
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
     };
     const char* const sk = smem + (buf ^ 1) * TBYTES;
     const char* const sv = smem + (2 + buf) * TBYTES;
-    const int kb = D == 64 ? ma_opaque(kbase) : kbase, vb = D == 64 ? ma_opaque(vbase) : vbase;      // (D = 64 has 168 registers: the swizzled addresses are made per tile)
+    const int kb = D == 64 || LATE ? ma_opaque(kbase) : kbase, vb = D == 64 || LATE ? ma_opaque(vbase) : vbase;      // (D = 64 has 168 registers: the swizzled addresses are made per tile)
     f32x16 acc[2] = {ma_zero(), ma_zero()};
     // (after the last tile the scores are those of an old buffer and nobody looks at them: a branch here would move the exponentials in front of it)
     ma_stream<NP, 4, v8>([&](auto x) { return TL::template row_frag<v8>(sk, kb, (x & 1) * 32, x >> 1); },
@@ -247,8 +248,10 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
     ma_stream<NP, 4, v8>([&](auto x) { return TL::template tr_frag<v8>(sv, vb, x % DT, x / DT * 16); },
                          [&](auto x, const v8 vf) {
                            rs.o[x % DT] = ma_mfma(vf, pf[x / DT], rs.o[x % DT]);
-                           ma_each<0, EPP>([&](auto y) __attribute__((always_inline)) { finish(MaIdx<decltype(x)::value * EPP + decltype(y)::value>{}, acc); });
+                           if constexpr (!LATE)
+                             ma_each<0, EPP>([&](auto y) __attribute__((always_inline)) { finish(MaIdx<decltype(x)::value * EPP + decltype(y)::value>{}, acc); });
                          });
+    if constexpr (LATE) ma_each<0, 32>([&](auto e) __attribute__((always_inline)) { finish(e, acc); });
     if (tn >= 0) {
       if (!(fln & 2)) mask(tn, buf ^ 1);
       rs.rise(mx);

@@ -144,7 +144,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   auto products = [&](const char* sk, const char* sv, const int k2, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
     s = ma_zero();
     dp = ma_zero();
-    ma_stream<2 * DK, REL && D == 128 ? 3 : 4, v8>([&](auto x) { return TL::template row_frag<v8>(x & 1 ? sv : sk, kbase, k2 * 32, x >> 1); },
+    const int kb = REL && D == 128 && (MODE & MA_WIDE) ? ma_opaque(kbase) : kbase;       // (registers: the swizzled addresses are made per half)
+    ma_stream<2 * DK, REL && D == 128 ? 3 : 4, v8>([&](auto x) { return TL::template row_frag<v8>(x & 1 ? sv : sk, kb, k2 * 32, x >> 1); },
                              [&](auto x, const v8 f) { if (x & 1) dp = ma_mfma(f, gf[x >> 1], dp); else s = ma_mfma(f, qf[x >> 1], s); });
   };
   int buf = 0;
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
             float ds = pr * (dp[r] - delta);
             if (!(fl & 2)) ds = (rg * 8 + e < ll) & (dk4[e] == dq) ? ds : 0.f;
             if (REL) dp[r] = ds;                                   // (kept for the diagonals)
-            if (MODE & MA_CAP) ds *= -4.f * sq * (1.f + sq);       // 1 - tanh^2, tanh = 1 + 2 sq
+            if (MODE & MA_CAP) ds *= sc.slope(sq);
             s[r] = ds * up;
           }
         }
@@ -480,7 +481,7 @@ __global__ __launch_bounds__(256, 2) void ma_dkv_kernel(const MgldMaskAttn p, co
             float sq = 0.f;
             float pr = sc.template prob<false>(s[r], at, rg * 8 + e, lse2[e] - pup, sq);
             float ds = pr * (dp[r] - delta[e]) * gup;
-            if (MODE & MA_CAP) ds *= -4.f * sq * (1.f + sq);
+            if (MODE & MA_CAP) ds *= sc.slope(sq);
             if (!(fl & 2)) {
               const int i = il + rg * 8 + e;
               const bool vis = jok & (i < p.Nq) & (j < bs.limit(p, bs.pos0 + i)) & (di[e] == dj);

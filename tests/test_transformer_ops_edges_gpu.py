@@ -124,3 +124,73 @@ def test_fp16_gradient_of_a_quiet_document(hip):
     rows = quiet[0].double().abs().sum(1).unflatten(1, (k.shape[2], -1)).sum(2)[:, None]
     _, _, grads = run(hip, q, k, v, do, kw)
     check("dk", grads[1][:, 150:], res["dk"], tol["dk"] + kw["scale"] * fl * rows)
+
+# ---- caps ------------------------------------------------------------------------------------------------------------------------------------------
+def cap_bounds(q, k, v, do, kw):
+    """fp64 results and bounds that do not grow with the cap.  A score's error: the product's, scale sum|q k| (d + 4) 2^-24 (the cap's slope is at most 1),
+    and the cap's own, at most 2^-20 |u| (below a quarter of the cap the odd series ends 2^-26 short and rounds six times, above it 1 - 2 / (1 + e^2x)
+    is off by 2^-23 of the cap <= 4.1 |u|).  A probability below fp32's smallest normal, 2^-126, may come out as zero."""
+    u, d, cap, scale = half_step(q.dtype), q.shape[3], kw["softcap"], kw["scale"]
+    Hk, G = k.shape[2], q.shape[2] // k.shape[2]
+    vis, dist = tr.visible(q.shape[0], q.shape[1], k.shape[1], kw["causal"], kw.get("docs"), None, None, kw.get("q_pos0"))
+    leaves = [x.double().requires_grad_() for x in (q, k, v)]
+    r = tr.attention(*leaves, vis, dist, scale, cap, kw["slopes"].double() if "slopes" in kw else None, kw["rel"].double() if "rel" in kw else None)
+    grads = torch.autograd.grad(r["o"], leaves, do.double())
+    with torch.no_grad():
+        tiny = torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps
+        P, kk, vv, dob = r["P"], r["k"].permute(0, 2, 1, 3), r["v"].permute(0, 2, 1, 3), do.double().permute(0, 2, 1, 3)
+        qa = q.double().abs().permute(0, 2, 1, 3)
+        es = float(torch.matmul(qa, kk.abs().transpose(2, 3)).max()) * scale * (d + 4) * 2.0 ** -24 + float(r["u"].abs().max()) * 2.0 ** -20 + 2.0 ** -18
+        E = 2 * es
+
+        def rows(x):
+            return x.permute(0, 2, 1, 3)
+
+        def fold(x):
+            return rows(x).unflatten(2, (Hk, G)).sum(3)
+
+        dP = torch.matmul(dob, vv.transpose(2, 3))
+        D = (P * dP).sum(-1, keepdim=True)
+        dS = P * (dP - D)
+        tdP = torch.matmul(dob.abs(), vv.abs().transpose(2, 3)) * (d + 4) * 2.0 ** -24
+        tD = (P * (tdP + E * dP.abs())).sum(-1, keepdim=True) * 1.02
+        dT = dS * (1 - (r["u"] / cap) ** 2)
+        tT = (P * (tdP + tD) + E * (dS.abs() + P * tD) + dS.abs() * 2.0 ** -20 + 2.0 ** -126 * r["vis"] * (dP - D).abs()) * 1.02 + u * dT.abs()
+        if q.dtype is F16:
+            tT = tT + r["vis"] * float(dP.abs().max()) * 2.0 ** -37          # (check_fp16_grads)
+        tol = {"o": u * r["o"].abs() + (u + E) * rows(torch.matmul(P, vv.abs())) * 1.02 + tiny, "lse": es + r["lse"].abs().nan_to_num(posinf=0) * 2.0 ** -21 + 2.0 ** -20,
+               "dq": u * grads[0].abs() + scale * rows(torch.matmul(tT, kk.abs())) * 1.02 + tiny,
+               "dk": u * grads[1].abs() + scale * fold(torch.matmul(tT.transpose(2, 3), qa)) * 1.02 + tiny,
+               "dv": u * grads[2].abs() + fold(torch.matmul(((u + E) * P + (2.0 ** -34 if q.dtype is F16 else 2.0 ** -126)).transpose(2, 3), dob.abs())) * 1.02 + tiny}
+    return {"o": r["o"].detach(), "lse": r["lse"].detach(), "dq": grads[0], "dk": grads[1], "dv": grads[2]}, tol
+
+
+@pytest.mark.parametrize("cap", [100.0, 150.0, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("name", ["cap", "cap_d64", "docs_causal_cap", "rel_causal_cap", "token", "d40_slopes", "rel_docs"])
+def test_caps_far_above_the_scores(hip, name, dt, cap):
+    q, k, v, do, kw = problem(name, dt, seed=15)
+    kw.pop("kv_len", None)
+    kw["softcap"] = cap
+    res, tol = cap_bounds(q, k, v, do, kw)
+    o, lse, grads = run(hip, q, k, v, do, kw)
+    check("o", o, res["o"], tol["o"])
+    check_lse(lse, res["lse"], tol["lse"])
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        check(n, x, res[n], tol[n])
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("name", ["cap", "cap_d64", "token"])
+def test_a_large_cap_that_bends(hip, name, dt):
+    """scores of several hundred under a cap of 200: both of the cap's forms, and the border between them (t / cap = 1/4) inside one tile"""
+    q, k, v, do, kw = problem(name, dt, seed=16)
+    kw.pop("kv_len", None)
+    q = (q.float() * 32).to(dt)
+    kw["softcap"] = 200.0
+    res, tol = cap_bounds(q, k, v, do, kw)
+    o, lse, grads = run(hip, q, k, v, do, kw)
+    check("o", o, res["o"], tol["o"])
+    check_lse(lse, res["lse"], tol["lse"])
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        check(n, x, res[n], tol[n])
