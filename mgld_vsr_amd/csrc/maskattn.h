@@ -197,7 +197,7 @@ struct Score {
   const float* rel;          // LDS: the head's distance row in log2 units, distance 0 at index reach + MA_PAD
   int reach;
   __device__ Score(const MgldMaskAttn& p, const int h, const float* srel) {
-    pre = CAP ? 2.f * MA_LOG2E * p.scale / p.softcap : p.scale * MA_LOG2E;
+    pre = CAP ? fminf(2.f * MA_LOG2E * p.scale / p.softcap, 3.4e38f) : p.scale * MA_LOG2E;       // (finite: a score of zero is zero under the smallest cap too)
     capA = CAP ? (WIDE ? 1.f : 2.f) * MA_LOG2E * p.softcap : 0.f;
     scale2 = p.scale * MA_LOG2E;
     slope2 = SLOPES ? p.slopes[h] * MA_LOG2E : 0.f;

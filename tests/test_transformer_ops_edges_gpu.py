@@ -194,3 +194,22 @@ def test_a_large_cap_that_bends(hip, name, dt):
     check_lse(lse, res["lse"], tol["lse"])
     for n, x in zip(("dq", "dk", "dv"), grads):
         check(n, x, res[n], tol[n])
+
+
+@pytest.mark.parametrize("cap", [1e-3, 1e-36, 1e-38, 1e-40])
+@pytest.mark.parametrize("name", ["cap", "cap_d64", "token"])
+def test_caps_far_below_the_scores(hip, name, cap):
+    """every score becomes +-cap: equal weights.  A zero query row has score 0 and the cap's full slope there; rows of zeros are the only ones with a gradient
+    for q.  (cap 1e-3: reference()'s bounds, the slope of small scores included)"""
+    q, k, v, do, kw = problem(name, BF16, seed=17)
+    kw.pop("kv_len", None)
+    q[:, 0] = 0
+    kw["softcap"] = cap
+    res, tol = reference(q, k, v, do, kw)
+    o, lse, grads = run(hip, q, k, v, do, kw)
+    check("o", o, res["o"], tol["o"])
+    check_lse(lse, res["lse"], tol["lse"])
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        assert torch.isfinite(x).all(), n
+    check("dv", grads[2], res["dv"], tol["dv"])
+    check("dq", grads[0][:, :1], res["dq"][:, :1], tol["dq"][:, :1])
