@@ -522,8 +522,8 @@ int64_t mgld_masked_attention_work(const MgldMaskAttn* p);
 int mgld_masked_attention(const MgldMaskAttn* p, void* stream);
 /* From the forward's o and lse: dV = P^T dO, dS = P (dO V^T - rowsum(dO o)), dRel = dS summed over rows, batch and equal distances,
  * dQ = scale dT K, dK = scale dT^T Q with dT = dS (1 - (u / softcap)^2); K / V gradients summed over the query heads that share them.
- * Queries that see nothing, keys at or past kv_len, padding rows (negative document) and keys ahead of every query may hold anything.  An infinity or NaN
- * in a row that takes part may spread to gradients of pairs it is not part of (tiles of 64 x 128 rows).
+ * Queries that see nothing and keys that no query sees may hold anything.  A key or value reaches dQ of the queries that see it and no other's; an
+ * infinity or NaN in q or dO of a query that sees something may reach dK / dV of keys it does not see (tiles of 64 x 128 rows).
  * (rowsum(dO o) is summed from P and dP in fp32: O is not read.)  Every sum has a fixed order.  Rows of dK / dV that no query sees are written as zeros. */
 int64_t mgld_masked_attention_grad_work(const MgldMaskAttn* p);
 int mgld_masked_attention_grad(const MgldMaskAttn* p, void* stream);

@@ -331,59 +331,105 @@ __device__ __forceinline__ void ma_load_rel(const MgldMaskAttn& p, const int h, 
 }
 
 // ---- exact row by row, for the few rows whose fast result is not finite: a product with a zero probability turns an infinity or NaN of a
-// value that the row does not see into NaN.  One wave recomputes row (b, h, i) from its visible keys alone: lanes are keys for the scores,
+// value (gradient: a key) that the row does not see into NaN.  One wave recomputes row (b, h, i) from its visible keys alone: lanes are keys for the scores,
 // then elements of d for the sum.
 template <typename T>
-__device__ __forceinline__ void ma_slow_row(const MgldMaskAttn& p, const int b, const int h, const int i) {
-  const int lane = threadIdx.x & 63, d = p.head_dim, hk = h / (p.heads / p.kv_heads);
-  const BatchSpan bs(p, b);
-  const int pos = bs.pos0 + i, lim = bs.limit(p, pos);
-  const int dq = p.doc_q ? p.doc_q[b * p.doc_q_sb + i] : 0;
-  const T* q = (const T*)p.Q + b * p.q_sb + (int64_t)i * p.q_si + h * p.q_sh;
-  const T* kb = (const T*)p.K + b * p.k_sb + hk * p.k_sh;
-  const T* vb = (const T*)p.V + b * p.v_sb + hk * p.v_sh;
-  const bool cap = p.softcap > 0.f;
-  auto score = [&](const int j) __attribute__((always_inline)) {          // log2 units; -inf where unseen
-    if (j >= lim || dq < 0 || (p.doc_k && p.doc_k[b * p.doc_k_sb + j] != dq)) return -MA_INF;
+struct ExactRow {
+  const MgldMaskAttn& p;
+  const T *q, *kb, *vb;
+  const int32_t* ids;        // the keys' document numbers
+  int b, h, i, d, pos, lim, doc;
+  __device__ ExactRow(const MgldMaskAttn& pp, const int bb, const int hh, const int ii) : p(pp), b(bb), h(hh), i(ii), d(pp.head_dim) {
+    const BatchSpan bs(p, b);
+    const int hk = h / (p.heads / p.kv_heads);
+    pos = bs.pos0 + i;
+    lim = bs.limit(p, pos);
+    doc = p.doc_q ? p.doc_q[b * p.doc_q_sb + i] : 0;
+    ids = p.doc_k ? p.doc_k + b * p.doc_k_sb : nullptr;
+    q = (const T*)p.Q + b * p.q_sb + (int64_t)i * p.q_si + h * p.q_sh;
+    kb = (const T*)p.K + b * p.k_sb + hk * p.k_sh;
+    vb = (const T*)p.V + b * p.v_sb + hk * p.v_sh;
+  }
+  __device__ __forceinline__ bool seen(const int j) const { return j < lim && doc >= 0 && !(ids && ids[j] != doc); }
+  // of a key that the row sees: the score in log2 units, and the cap's slope there
+  __device__ __forceinline__ float score(const int j, float& slope) const {
     const T* k = kb + (int64_t)j * p.k_si;
     float t = 0.f;
     for (int e = 0; e < d; ++e) t += (float)q[e] * (float)k[e];
     t *= p.scale;
-    if (cap) {
+    slope = 1.f;
+    if (p.softcap > 0.f) {
       const float x = t / p.softcap;
-      t = fabsf(x) < 0.25f ? t * ma_tanh_ratio(x * x) : p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * MA_LOG2E))));
+      const bool near = fabsf(x) < 0.25f;
+      const float r = ma_tanh_ratio(x * x), th = near ? x * r : 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * (2.f * MA_LOG2E)));
+      t = near ? t * r : p.softcap * th;
+      slope = 1.f - th * th;
     }
     const int delta = j - pos;
     if (p.slopes) t -= p.slopes[h] * fabsf((float)delta);
     if (p.rel) t += p.rel[(int64_t)h * (2 * p.reach + 1) + min(max(delta, -p.reach), p.reach) + p.reach];
     return t * MA_LOG2E;
-  };
-  auto seen = [&](const int j) __attribute__((always_inline)) { return j < lim && dq >= 0 && !(p.doc_k && p.doc_k[b * p.doc_k_sb + j] != dq); };
-  float m = -MA_INF;
-  for (int j = lane; j < lim; j += 64) m = fmaxf(m, score(j));
-  m = wave_max(m);
-  if (m == -MA_INF) m = 0.f;
-  float l = 0.f, acc0 = 0.f, acc1 = 0.f;
-  for (int j0 = 0; j0 < lim; j0 += 64) {
-    const int j = j0 + lane;
-    const bool s = seen(j);
-    const float pr = s ? __builtin_amdgcn_exp2f(score(j) - m) : 0.f;
-    l += pr;
+  }
+  // sum over the keys of [j0, j0 + 64) that are seen of w (lane's key j0 + lane) times their rows at `rows`: a lane's elements lane, lane + 64
+  __device__ __forceinline__ void add(const int j0, const float w, const bool s, const T* rows, const int64_t stride, float& a0, float& a1) const {
+    const int lane = threadIdx.x & 63;
     unsigned long long todo = __ballot(s);
     while (todo) {
       const int c = __builtin_ctzll(todo);
       todo &= todo - 1;
-      const float pc = __shfl(pr, c, 64);
-      const T* v = vb + (int64_t)(j0 + c) * p.v_si;
-      if (lane < d) acc0 += pc * (float)v[lane];
-      if (lane + 64 < d) acc1 += pc * (float)v[lane + 64];
+      const float wc = __shfl(w, c, 64);
+      const T* r = rows + (int64_t)(j0 + c) * stride;
+      if (lane < d) a0 += wc * (float)r[lane];
+      if (lane + 64 < d) a1 += wc * (float)r[lane + 64];
     }
+  }
+  __device__ __forceinline__ void put(void* out, const int64_t sb, const int64_t si, const int64_t sh, const float a0, const float a1) const {
+    const int lane = threadIdx.x & 63;
+    T* const o = (T*)out + b * sb + (int64_t)i * si + h * sh;
+    if (lane < d) o[lane] = (T)a0;
+    if (lane + 64 < d) o[lane + 64] = (T)a1;
+  }
+};
+template <typename T>
+__device__ __forceinline__ void ma_slow_row(const MgldMaskAttn& p, const int b, const int h, const int i) {
+  const ExactRow<T> row(p, b, h, i);
+  const int lane = threadIdx.x & 63;
+  float m = -MA_INF, sl;
+  for (int j = lane; j < row.lim; j += 64)
+    if (row.seen(j)) m = fmaxf(m, row.score(j, sl));
+  m = wave_max(m);
+  if (m == -MA_INF) m = 0.f;
+  float l = 0.f, a0 = 0.f, a1 = 0.f;
+  for (int j0 = 0; j0 < row.lim; j0 += 64) {
+    const bool s = row.seen(j0 + lane);
+    const float pr = s ? __builtin_amdgcn_exp2f(row.score(j0 + lane, sl) - m) : 0.f;
+    l += pr;
+    row.add(j0, pr, s, row.vb, p.v_si, a0, a1);
   }
   l = wave_sum(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
-  if (lane < d) o[lane] = (T)(acc0 * inv);
-  if (lane + 64 < d) o[lane + 64] = (T)(acc1 * inv);
+  row.put(p.O, p.o_sb, p.o_si, p.o_sh, a0 * inv, a1 * inv);
+}
+// dQ of the row, from its lse (log2 units) and D
+template <typename T>
+__device__ __forceinline__ void ma_slow_dq(const MgldMaskAttn& p, const int b, const int h, const int i, const float lse2, const float delta) {
+  const ExactRow<T> row(p, b, h, i);
+  const int lane = threadIdx.x & 63;
+  const T* const g = (const T*)p.dO + b * p.do_sb + (int64_t)i * p.do_si + h * p.do_sh;
+  float a0 = 0.f, a1 = 0.f;
+  for (int j0 = 0; j0 < row.lim; j0 += 64) {
+    const int j = j0 + lane;
+    const bool s = row.seen(j);
+    float dt = 0.f;
+    if (s) {
+      const T* v = row.vb + (int64_t)j * p.v_si;
+      float dp = 0.f, sl;
+      for (int e = 0; e < row.d; ++e) dp += (float)g[e] * (float)v[e];
+      dt = __builtin_amdgcn_exp2f(row.score(j, sl) - lse2) * (dp - delta) * sl;
+    }
+    row.add(j0, dt, s, row.kb, p.k_si, a0, a1);
+  }
+  row.put(p.dQ, p.dq_sb, p.dq_si, p.dq_sh, a0 * p.scale, a1 * p.scale);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------

@@ -282,7 +282,14 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     buf ^= 1;
     t = tn; fl = fln;
   }
-  if (rok) {
+  float z = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z += o[dt][r] * 0.f;
+  const unsigned long long bz = __ballot(z != z);      // an infinity or NaN came in: perhaps by a key that the row does not see
+  unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
+  if (rok && !((bad >> l31) & 1)) {
     const float f = p.scale / up;
     T* const out = (T*)p.dQ + b * p.dq_sb + (int64_t)i * p.dq_si + h * p.dq_sh;
 #pragma unroll
@@ -311,6 +318,11 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
       for (int ww = 0; ww < 4; ++ww) f += s0[ww * (32 * 33 + nrel) + e];
       out[e] = f;
     }
+  }
+  while (bad) {
+    const int r = __builtin_ctz(bad);
+    bad &= bad - 1;
+    if (iw + r < p.Nq) ma_slow_dq<T>(p, b, h, iw + r, __shfl(lse2, r, 64), __shfl(delta, r, 64));
   }
 }
 

@@ -1291,7 +1291,8 @@ def masked_attention_grad(q, k, v, o, lse, do, *, scale=None, causal=False, soft
                           q_pos0=None, dq=None, dk=None, dv=None, drel=None, work=None):
     """Gradient of masked_attention, called with the same options, its results o and lse, and do = the gradient of o.  (do . o is summed again
     from the probabilities in fp32: the rounded o would cost the gradients precision, so o itself is only checked.)
-    Queries that see nothing, keys past kv_len, padding and keys ahead of every query may hold anything; a NaN in a row that takes part may spread further.
+    Queries that see nothing and keys that no query sees may hold anything.  A NaN in a key or value reaches dq of the queries that see it alone; one in q or do
+    of a query that sees something may reach dk / dv of keys it does not see.
     -> (dq, dk, dv, drel): dk / dv summed over the query heads that share them, zeros where no query sees the key; drel fp32 like rel (None
     without rel).  Sums have a fixed order: equal calls give equal bits."""
     what = "masked_attention_grad"

@@ -213,3 +213,61 @@ def test_caps_far_below_the_scores(hip, name, cap):
         assert torch.isfinite(x).all(), n
     check("dv", grads[2], res["dv"], tol["dv"])
     check("dq", grads[0][:, :1], res["dq"][:, :1], tol["dq"][:, :1])
+
+# ---- what a mask hides, gradient ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("what", ["a document without queries", "documents in between", "ahead of its document's queries", "two documents' tiles"])
+@pytest.mark.parametrize("dt,d", [(F16, 64), (BF16, 128)])
+def test_keys_that_no_query_sees_hold_anything(hip, dt, d, what, bad):
+    g = gen(44)
+    q, k, v, do = (randn(g, 2, 150, 2, d).to(dt) for _ in range(4))
+    kw = dict(causal=False, scale=d ** -0.5, softcap=0.0, q_pos0=0)
+    dq = torch.zeros(2, 150, dtype=torch.int32)
+    dk, gone = dq.clone(), torch.zeros(2, 150, dtype=torch.bool)
+    if what == "a document without queries":
+        dk[1, 40:71] = 9
+        gone[1, 40:71] = True
+    elif what == "documents in between":                                  # the missing number lies between two that the block has
+        dq[:, 70:] = dk[:, 70:] = 12
+        dk[:, 60:90] = 9
+        gone[:, 60:90] = True
+    elif what == "ahead of its document's queries":                       # document 1's queries end before its last keys begin
+        kw["causal"] = True
+        dq[:, 30:50] = 1
+        dk[:, 20:50] = 1
+        dk[:, 100:110] = 1
+        gone[:, 100:110] = True
+    else:
+        kw["causal"] = True
+        dq[0, 64:] = dk[0, 64:] = 1
+        dk[0, 120:130], dk[1, 3:5] = 4, 4
+        gone[0, 120:130], gone[1, 3:5] = True, True
+    kw["docs"] = (dq, dk)
+    vis, _ = tr.visible(2, 150, 150, kw["causal"], kw["docs"], None, None, 0)
+    assert torch.equal(gone, ~vis.any(1))
+    res, tol = reference(q, k, v, do, kw)
+    k[gone], v[gone] = bad, bad
+    o, lse, grads = run(hip, q, k, v, do, kw)
+    check("o", o, res["o"], tol["o"])
+    check_lse(lse, res["lse"], tol["lse"])
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        check(n, x, res[n], tol[n])
+    assert not grads[1].cpu()[gone].any() and not grads[2].cpu()[gone].any()
+
+
+@pytest.mark.parametrize("name,dt,key", [("docs", F16, 100), ("docs_causal_cap", BF16, 60), ("prefix", F16, 155), ("d40_slopes", BF16, 50), ("rel_causal_cap", F16, 130),
+                                         ("tokens", BF16, 698)])
+def test_dq_depends_on_what_its_row_sees_alone(hip, name, dt, key):
+    """a NaN or infinity in a key or value reaches dQ of the rows that see it, and no other row's"""
+    q, k, v, do, kw = problem(name, dt, seed=18)
+    res, tol = reference(q, k, v, do, kw)
+    vis, _ = tr.visible(q.shape[0], q.shape[1], k.shape[1], kw["causal"], kw.get("docs"), kw.get("prefix"), kw.get("kv_len"), kw.get("q_pos0"))
+    for x, bad in ((k, float("nan")), (v, float("inf"))):
+        kb, vb = k.clone(), v.clone()
+        (kb if x is k else vb)[:, key] = bad
+        _, _, grads = run(hip, q, kb, vb, do, kw)
+        blind = ~vis[:, :, key]
+        m = blind[:, :, None, None].expand_as(res["dq"])
+        check("dq blind", torch.where(m, grads[0].cpu().double(), res["dq"]), res["dq"], tol["dq"])
+        assert bool(blind.any()) and bool((~blind).any())
+        assert not torch.isfinite(grads[0].cpu()[~m]).all()
