@@ -6,8 +6,9 @@
 //  * Scores are computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16): a lane holds 16 keys of ONE query row per 32-key half tile, so the row
 //    maximum and sum are lane-local plus one exchange with lane ^ 32, and the probabilities are the second product's operand as they lie,
 //    O^T = V^T P^T.  V stays row-major in LDS; its transposed fragments come from ds_read_b64_tr_b16.
-//  * One pass with the running maximum (it moves only when a score exceeds it by 2^6, so the accumulator is rarely rescaled: P <= 2^6 fits fp16)
-//    and the sum in fp32.
+//  * One pass with the running maximum (it moves only when a score exceeds it by 2^6, so the accumulator is rarely rescaled) and the sum in fp32.  In fp16
+//    probabilities are held as 2^9 P <= 2^15: of many small ones beside a large one each is off by at most 2^-34 of it (as P, by 2^-25: half of the sum of
+//    2^17 keys at 2^-24.6).
 //  * Which tiles a block visits, and which of them need no mask, is decided 64 tiles at a time: lane l judges tile t0 + l and two
 //    ballots give the bit masks.  A causal, prefix, length or document mask costs skipped tiles nothing and full tiles nothing.
 //
@@ -41,8 +42,9 @@ __global__ __launch_bounds__(64) void ma_doc_tiles_kernel(const int32_t* dk, con
 
 // a query row's running maximum (log2 units), sum and accumulators
 constexpr float MA_SLACK = 6.f;        // the maximum moves when a score exceeds it by this much: probabilities stay below 2^6
-template <int DT>
+template <typename T, int DT>
 struct RowState {
+  static constexpr float LIFT = __is_same(T, f16) ? 9.f : 0.f;       // probabilities are held as 2^LIFT P
   f32x16 o[DT];
   float m, l;
   __device__ RowState() : m(-MA_INF), l(0.f) {
@@ -63,7 +65,8 @@ struct RowState {
       m = mn;
     }
   }
-  __device__ __forceinline__ float base() const { return m == -MA_INF ? 0.f : m; }
+  __device__ __forceinline__ float base() const { return m == -MA_INF ? 0.f : m - LIFT; }
+  __device__ __forceinline__ float unit() const { return m - LIFT; }       // what o and l are relative to (-inf: nothing was visible)
 };
 
 // masks a 32-key half of the scores: keys k0 + ma_row(r) + 4 half at or past `lim`, or of another document than dq
@@ -168,7 +171,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
     dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, bs.len - k0, lds0 + (2 + buf) * TBYTES, flags & 4, [&](const int r) { return ids[r] < 0; });
   };
 
-  RowState<DT> rs;
+  RowState<T, DT> rs;
   const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
   constexpr int NP = 2 * DK, EPP = 32 / NP;            // products of a 64-key tile (scores, and P V as many), scores per product
   constexpr bool LATE = D == 128 && (MODE & MA_WIDE) && (MODE & (MA_REL | MA_SLOPES));       // the next scores after the second product, not beside it (registers)
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   const unsigned long long bz = __ballot(z != z);      // an infinity or NaN came in
   unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
   if (i < p.Nq) {
-    if (p.lse && lhi == 0) p.lse[((int64_t)b * p.heads + h) * p.Nq + i] = l == 0.f ? -MA_INF : (rs.m + __builtin_amdgcn_logf(l)) * MA_LN2;
+    if (p.lse && lhi == 0) p.lse[((int64_t)b * p.heads + h) * p.Nq + i] = l == 0.f ? -MA_INF : (rs.unit() + __builtin_amdgcn_logf(l)) * MA_LN2;
     if (!((bad >> l31) & 1)) {
       T* const o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
 #pragma unroll
@@ -372,7 +375,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     dv.load(Vp, (int64_t)k0 * p.v_si * 2, p.v_si, g.lim_max - k0, a + TBYTES);
     if (docs) ma_dma4(lds_doc + buf * MA_KT * 4, lane, min(KH, g.lim_max - k0), p.doc_k + b * p.doc_k_sb + k0);
   };
-  RowState<DT> rs;
+  RowState<T, DT> rs;
   const int kbase = TL::row_base(lane), vbase = TL::tr_base(lane);
   int fl = 0, buf = 0;
   int t = advance(fl);
@@ -417,7 +420,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
   // ---- the four waves' states meet: o * 2^(m_w - M)
   const float l = rs.l + __shfl_xor(rs.l, 32, 64);
   __syncthreads();                                       // every wave is done with its tiles
-  if (lhi == 0) { sml[wave * 64 + l31] = rs.m; sml[wave * 64 + 32 + l31] = l; }
+  if (lhi == 0) { sml[wave * 64 + l31] = rs.unit(); sml[wave * 64 + 32 + l31] = l; }
   float* const so = (float*)smem + wave * 32 * D;        // [32 rows][D] fp32 = the wave's two tiles' bytes
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)

@@ -271,3 +271,25 @@ def test_dq_depends_on_what_its_row_sees_alone(hip, name, dt, key):
         check("dq blind", torch.where(m, grads[0].cpu().double(), res["dq"]), res["dq"], tol["dq"])
         assert bool(blind.any()) and bool((~blind).any())
         assert not torch.isfinite(grads[0].cpu()[~m]).all()
+
+# ---- many small probabilities ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("Nq,H", [(1, 1), (130, 40)])
+@pytest.mark.parametrize("below", [17.0, 20.4, 24.6])
+def test_many_small_probabilities_beside_a_large_one(hip, below, Nq, H, dt):
+    """2^17 keys whose probabilities are 2^-below of the first one's: their sum counts.  Rounded to fp16 as P 2^9, each is off by at most 2^-34 of the largest
+    (half a smallest step, 2^-25, over 2^9; the running maximum is at most 2^6 below the largest score) beside its relative half step"""
+    N, d = 1 << 17, 64
+    q, k, v = torch.zeros(1, Nq, H, d), torch.zeros(1, N, 1, d), torch.ones(1, N, 1, d)
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = 8.0, below * math.log(2.0), 0.0
+    v[:, 1:, :, 1] = 0.5
+    q, k, v = (x.to(dt) for x in (q, k, v))
+    kw = dict(scale=0.125, causal=False, softcap=0.0, q_pos0=0)
+    s = float(k[0, 0, 0, 0].double()) * 8.0 * 0.125
+    P = math.exp(-s) / (1 + (N - 1) * math.exp(-s))
+    ref = torch.full((1, Nq, H, d), (N - 1) * P, dtype=torch.float64)
+    ref[..., 1] *= 0.5
+    E = 2 * (s * (d + 4) * 2.0 ** -24 + 2.0 ** -20)
+    o, lse = hip.masked_attention(q.to(DEV), k.to(DEV), v.to(DEV), **kw)
+    # (the sum of N fp32 terms of one size: 2^-24 of it a step, at most N / 64 steps in a lane's chain)
+    check("o", o, ref, (2 * half_step(dt) + E + N / 64 * 2.0 ** -24) * ref + (N * 2.0 ** -34 if dt is F16 else 0.0))
