@@ -14,11 +14,12 @@ LIB = os.path.join(HERE, "libmgld_hip.so")
 STAMP = os.path.join(HERE, "csrc", ".build_stamp")
 SOURCES = ["runtime.hip", "igemm.hip", "conv3q.hip", "ppgemm.hip", "conv3r.hip", "pptconv.hip", "norm.hip", "attention.hip", "elementwise.hip", "raft.hip", "hpenc.hip",
            "qkrope.hip", "maskattn.hip", "maskattn_grad.hip", "relbias.hip"]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result"]
-# no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms give wrong results now and then on this hardware.  norm.hip keeps it:
-# without it the compiler contracts the normalisations' products differently, and the recorded results of the samplers move
+# no packed fp32 arithmetic (v_pk_add / mul / fma_f32), in any source: the compiler makes it by itself from ordinary float code, and some of its forms
+# have given wrong results now and then on the machines this runs on.  (No kernel here was seen to.)
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-PACKED_FP32 = ("norm.hip",)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wno-unused-result"] + NO_PACKED_FP32
+# a source whose roundings the samplers amplify writes each of them out (fmaf, or product and sum): nothing is left to the compiler's contraction
+SOURCE_FLAGS = {"norm.hip": ["-ffp-contract=off"]}
 
 
 def _hipcc():
@@ -28,8 +29,8 @@ def _hipcc():
     raise RuntimeError("hipcc not found")
 
 
-def _flags(source):
-    return FLAGS if source in PACKED_FP32 else FLAGS + NO_PACKED_FP32
+def flags(source):
+    return FLAGS + SOURCE_FLAGS.get(source, [])
 
 
 def _file_digest(paths):
@@ -38,7 +39,7 @@ def _file_digest(paths):
         with open(f, "rb") as fh:
             h.update(fh.read())
     for f in paths:
-        h.update(" ".join(_flags(os.path.basename(f))).encode())
+        h.update(" ".join(flags(os.path.basename(f))).encode())
     return h.hexdigest()
 
 
@@ -68,7 +69,7 @@ def build(force=False, verbose=True):
         ostamp = obj + ".stamp"
         if not force and os.path.exists(obj) and os.path.exists(ostamp) and open(ostamp).read().strip() == odig:
             continue
-        cmd = [hipcc] + _flags(s) + ["-c", os.path.join(CSRC, s), "-o", obj]
+        cmd = [hipcc] + flags(s) + ["-c", os.path.join(CSRC, s), "-o", obj]
         if verbose:
             print("[mgld build]", " ".join(cmd), flush=True)
         procs.append((s, ostamp, odig, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
