@@ -219,6 +219,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   // one tile: its probabilities beside the products of the next tile's scores, then its second product beside the next scores' cap, bias and
   // maximum.  Each product is followed by the arithmetic of EPP scores, in this order, so that the matrix pipe and the vector pipe work on
   // one wave at the same time.
+  ma_loads_landed();
   while (t >= 0) {
     ma_dma_wait();
     __syncthreads();                                   // the next K and this V have landed everywhere, and everyone is done with the other buffers
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   while (bad) {
     const int r = __builtin_ctz(bad);
     bad &= bad - 1;
-    if (iw + r < p.Nq) ma_slow_row<T>(p, b, h, iw + r);
+    if (iw + r < p.Nq) ma_slow_row<T>(D == 128 ? ma_late_args() : p, b, h, iw + r);
   }
 }
 

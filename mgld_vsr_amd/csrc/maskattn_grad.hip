@@ -322,7 +322,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   while (bad) {
     const int r = __builtin_ctz(bad);
     bad &= bad - 1;
-    if (iw + r < p.Nq) ma_slow_dq<T>(p, b, h, iw + r, __shfl(lse2, r, 64), __shfl(delta, r, 64));
+    if (iw + r < p.Nq) ma_slow_dq<T>(ma_late_args(), b, h, iw + r, __shfl(lse2, r, 64), __shfl(delta, r, 64));
   }
 }
 
