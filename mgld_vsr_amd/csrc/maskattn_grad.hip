@@ -154,6 +154,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
     int fl = 0, fln = 0;
     int t = advance(fl);
     if (t >= 0) load_tile(t, buf, fl);
+    ma_loads_landed();
     while (t >= 0) {
       ma_dma_wait();
       __syncthreads();
@@ -206,6 +207,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   int fl = 0, fln = 0;
   int t = advance(fl);
   if (t >= 0) load_tile(t, buf, fl);
+  ma_loads_landed();
   while (t >= 0) {
     ma_dma_wait();
     __syncthreads();
