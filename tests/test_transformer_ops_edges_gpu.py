@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import transformer as tr
-from test_transformer_ops_gpu import ATT, BF16, DEV, F16, check, check_lse, docs_of, gen, half_step, on_gpu, problem, randn, reference
+from test_transformer_ops_gpu import ATT, BF16, DEV, F16, check, check_lse, gen, half_step, on_gpu, problem, randn, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -271,6 +271,28 @@ def test_dq_depends_on_what_its_row_sees_alone(hip, name, dt, key):
         check("dq blind", torch.where(m, grads[0].cpu().double(), res["dq"]), res["dq"], tol["dq"])
         assert bool(blind.any()) and bool((~blind).any())
         assert not torch.isfinite(grads[0].cpu()[~m]).all()
+
+@pytest.mark.parametrize("cap", [40.0, 300.0, 1e5])
+@pytest.mark.parametrize("name,dt", [("docs_causal_cap", F16), ("cap_d64", BF16)])
+def test_row_by_row_forms_under_any_cap(hip, name, dt, cap):
+    """one row's NaN key and value leave the other rows of its tile to their visible keys, one by one: o and dq there keep the cap's bounds"""
+    q, k, v, do, kw = problem(name, dt, seed=19)
+    q = (q.float() * 8).to(dt)
+    if "docs" not in kw:                                    # key 30 is seen by the rows of its document alone
+        ids_q, ids_k = torch.zeros(q.shape[:2], dtype=torch.int32), torch.zeros(k.shape[:2], dtype=torch.int32)
+        ids_q[:, 7], ids_k[:, 25:33] = 1, 1
+        kw["docs"] = (ids_q, ids_k)
+    key = 60 if name == "docs_causal_cap" else 30
+    kw["softcap"] = cap
+    res, tol = cap_bounds(q, k, v, do, kw)
+    blind = ~tr.visible(q.shape[0], q.shape[1], k.shape[1], kw["causal"], kw["docs"], None, None, kw.get("q_pos0"))[0][:, :, key]
+    k[:, key], v[:, key] = float("nan"), float("nan")
+    o, _, grads = run(hip, q, k, v, do, kw)
+    m = blind[:, :, None, None].expand_as(res["o"])
+    assert bool(m.any()) and not bool(m.all())
+    for n, x in (("o", o), ("dq", grads[0])):
+        check(n, torch.where(m, x.cpu().double(), res[n]), res[n], tol[n])
+
 
 # ---- many small probabilities ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [F16, BF16])
