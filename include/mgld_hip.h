@@ -497,13 +497,13 @@ int mgld_qk_norm_rope_grad(const MgldQkRope* p, void* stream);
  *   visible: j < len_b, and (causal: j <= p_i or j < prefix[b]), and (documents: doc_q[i] == doc_k[j] >= 0)
  *   o = sum_visible softmax(s) v,  lse = log sum_visible exp(s);   a query that sees nothing: o = 0, lse = -inf, and no gradient.
  * A value or key that a query does not see never reaches that query's result, whatever it holds (infinities, NaN).
- * heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads). */
+ * heads % kv_heads == 0: query head h reads key / value head h / (heads / kv_heads).  Row strides (*_si) of what is read: below 2^23 elements. */
 typedef struct MgldMaskAttn {
   const void* Q; const void* K; const void* V; void* O;
   float* lse;                       /* [batch, heads, Nq] contiguous, or NULL (forward only)                                */
   int64_t q_sb, q_si, q_sh, k_sb, k_si, k_sh, v_sb, v_si, v_sh, o_sb, o_si, o_sh;
   const float* slopes;              /* [heads] or NULL                                                                      */
-  const float* rel;                 /* [heads, 2 * reach + 1] or NULL; reach <= 1024; not together with slopes               */
+  const float* rel;                 /* [heads, 2 * reach + 1] or NULL; reach <= 1024; not together with slopes.  Gradient: (heads / kv_heads) * (2 reach + 129) <= 23552 */
   const int32_t* doc_q; const int32_t* doc_k;   /* [batch, Nq], [batch, Nkv], unit stride, both or neither                  */
   const int32_t* prefix;            /* [batch] or NULL; needs causal                                                        */
   const int32_t* kv_len;            /* [batch] or NULL                                                                      */

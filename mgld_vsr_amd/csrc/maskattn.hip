@@ -13,11 +13,12 @@
 //    ballots give the bit masks.  A causal, prefix, length or document mask costs skipped tiles nothing and full tiles nothing.
 //
 // Bounds and figures (4 d products per visible pair; a large matrix product reaches 1400 TFLOP/s):
-//  * many rows, d = 128: 880-905 TFLOP/s on full tiles, 730-750 under a cap (three transcendentals per score: the vector pipe is active 70 % of the
-//    cycles, the matrix pipe 34 %), ~740 at d = 64; ~10 us a launch beside that.  8192 tokens, 32 / 8 heads of 128, causal, cap 50: 714 us.  128 rows a block =
+//  * many rows, d = 128: 880-905 TFLOP/s on full tiles, 750-780 under a cap (three transcendentals per score), ~740 at d = 64; ~10 us a launch beside that.
+//    8192 tokens, 32 / 8 heads of 128, causal, cap 50: 707 us.  Neither pipe is full there: the vector pipe is active 72 % of the cycles, the matrix pipe 35 %, and waves
+//    wait 21 % of theirs: the chain from a score over its exponentials to the second product, with two waves per SIMD to hide it.  128 rows a block =
 //    two blocks per CU (three at d = 64), so one's barrier is the other's work.
 //    Keeping unscaled scores (32 of 340 vector instructions fewer per tile) gained 0.8 % and spilled at d = 64; one m0 write for several DMA pieces: nothing.
-//  * few rows: HBM.  16 sequences of up to 32768 cached tokens, 8 key heads of 128 (1.40 GB): 242 + 5 us, 5.6 TB/s.
+//  * few rows: HBM.  16 sequences of up to 32768 cached tokens, 8 key heads of 128 (1.40 GB): 241 + 5 us, 5.6 TB/s.
 #include "maskattn.h"
 
 namespace {
@@ -498,7 +499,11 @@ __global__ __launch_bounds__(64) void ma_join_kernel(const MgldMaskAttn p, const
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 struct Plan { bool split; int nsplit, nrb; };
-// few rows: when one block per 128 rows would leave most of the card idle and there are keys to share out
+// few rows: when one block per 128 rows would leave most of the card idle and there are keys to share out.  Row blocks | split, us (fp16, causal):
+//   32 / 8 heads of 128, 512 keys: 16 rows 20.1 | 13.4, 17 rows 20.0 | 13.5, 128 rows 19.4 | 16.4;  16 sequences of 2048 keys: 16 rows 99 | 55, 17 rows 106 | 75
+//   (from 17 rows on these count as many rows, and lose a third);  16 heads of 64, 4096 keys: 17 rows 109 | 17, 128 rows 90 | 21, 512 rows 88 | 35;
+//   4 heads of 128, 4096 keys: 512 rows 114 | 34, 2048 rows 114 | 60;  16 heads of 64, 77 keys: 8 rows 7.3 | 7.0, 16 rows 7.3 | 8.4;  2 heads of 64, 300 rows: 960 keys 25.5 | 12.4
+//   (row blocks: fewer than 16 tiles), 1024 keys 27.2 | 12.5.  Both borders are on the safe side of the crossing, not at it.
 Plan ma_plan(const MgldMaskAttn* p) {
   Plan pl{false, 1, 1};
   const int G = p->heads / p->kv_heads, nt = ma_tiles(p->Nkv);

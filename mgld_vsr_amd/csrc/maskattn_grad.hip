@@ -11,9 +11,9 @@
 //    blocks wholly beyond the reach only add to the two end sums.
 //  * ma_dkv_kernel, per 128 keys of a key head: S = Q K^T and dP = dO V^T (a lane holds query rows of ONE key), dV^T += dO^T P, dK^T += Q^T dT over
 //    all query heads of the group.  Where that gives too few blocks, the (head, tile) list is dealt to `nsp` blocks whose fp32 sums are added.
-// Bounds and figures: 2 x 2048 tokens, 16 / 4 heads of 128, causal with a prefix: dQ 160 us, dK / dV 146 + 13 us (forward 66).  At d = 128 the LDS reads of 32 rows or keys
+// Bounds and figures: 2 x 2048 tokens, 16 / 4 heads of 128, causal with a prefix: dQ 157 us, dK / dV 148 + 13 us (forward 66).  At d = 128 the LDS reads of 32 rows or keys
 // per wave take as long as the products (wider waves need more registers than there are), and two waves per SIMD hide little of the scores'
-// arithmetic behind them.  With a learned bias (4 x 1024 tokens, 16 heads of 64): dQ 101 us, dK / dV 84 us (forward 40): the diagonals pass through LDS.
+// arithmetic behind them.  With a learned bias (4 x 1024 tokens, 16 heads of 64): dQ 103 us, dK / dV 84 us (forward 40): the diagonals pass through LDS.
 // fp16 operands have 5 exponent bits: dT is scaled by powers of two before its rounding, per row in ma_dq, by one number for the call in ma_dkv.  The scale
 // comes from dS itself: |dS| = P |dP - D| <= max(P |dP|) + |D|, which the pass for D has at hand (one more maximum per score), so that bound goes to
 // 2^13 .. 2^14 whatever the sizes of dO and V: nothing overflows, and what is rounded to a subnormal lies 2^27 below the largest.  P is rounded as 2^10 P there.

@@ -113,8 +113,8 @@ __device__ __forceinline__ void gn_group_stats(const double* __restrict__ gs, in
 // ---- the same from per-CHANNEL fp32 tile sums (kind 1: written by the ping-pong GEMM family's epilogue, MgldIGemm.gn_part):
 // part[frame * chunks + chunk][2][C] floats (sum row, sumsq row).  Only the groups of the caller's channel window [c_off, c_off + Cw) are
 // computed: threads run along channels (coalesced rows of part[], the chunk loads independent), the per-channel totals meet in LDS
-// (chs[2][Cw] DOUBLES, caller-provided) and one thread per group adds its cg channels in fp64.  The cross-chunk totals are fp64 too
-// (round 5): at the VAE's 256^2 / 512^2 planes a channel has 128-1024 tile sums, and for a channel with |mean| >> std the
+// (chs[2][Cw] DOUBLES, caller-provided) and one thread per group adds its cg channels in fp64.  The cross-chunk totals are fp64 too:
+// at the VAE's 256^2 / 512^2 planes a channel has 128-1024 tile sums, and for a channel with |mean| >> std the
 // variance q/n - mean^2 cancels — 1e-6 of relative error in the fp32 running totals was a percent of the variance.
 __device__ __forceinline__ void gn_group_stats_pc(const float* __restrict__ part, int chunks, int C, int c_off, int Cw, int rows, int cg,
                                                   float eps, float (*st)[2], double* __restrict__ chs) {
@@ -458,8 +458,8 @@ extern "C" int mgld_gn_chunks(int rows_per_frame) {
 
 // LDS of the kernels that keep [rows per pass][channel window][2] floats: a block of window Cw runs rpi(Cw) = 256 / (Cw / 8) row slots,
 // and rpi(Cw) * Cw is NOT monotonic in Cw — the last, narrower window of a ragged split can need more than the full ones
-// (C = 1280 in windows of 440: the 400-channel tail runs 5 slots x 400 = 2000 channel slots, the full windows 4 x 440 = 1760;
-// ADVICE round 4) — so the launch is sized for the larger of the two window widths it contains.
+// (C = 1280 in windows of 440: the 400-channel tail runs 5 slots x 400 = 2000 channel slots, the full windows 4 x 440 = 1760) —
+// so the launch is sized for the larger of the two window widths it contains.
 static size_t row_slots_lds_one(int Cw) {
   const int NV = Cw >> 3;
   const int rpi = NV >= 256 ? 1 : 256 / NV;

@@ -321,7 +321,9 @@ template <typename T, int P, int LG, bool IL>
 int qr_launch(const MgldQkRope& p, const bool grad, hipStream_t st) {
   constexpr int NG = 256 / LG;
   if (!grad) {
-    // many rows: a group walks several heads of its token (sines once per token); few rows: one head per group, heads over blockIdx.y
+    // many rows: a group walks several heads of its token (sines once per token); few rows: one head per group, heads over blockIdx.y.  Few | many, us:
+    // 40 heads of 128 bf16: 256 rows 4.5 | 7.6, 1024 9.4 | 9.3, 2048 15.2 | 10.9, 4096 27.5 | 19.3, 16384 86 | 53;  32 of 64 fp16: 2048 6.7 | 8.2, 3000 9.3 | 9.0, 4096 10.7 | 9.6;
+    // 10 of 64: 2048 4.7 | 8.4, 4096 6.4 | 9.5, 6000 8.9 | 9.7, 8192 10.2 | 10.0.  4096 lies between the crossings (1000 .. 8000, by the heads).
     const int H = p.q.heads + p.k.heads;
     int GT = NG;
     if (p.rows >= 4096) while (GT > 1 && GT * 4 > H) GT /= 2;
