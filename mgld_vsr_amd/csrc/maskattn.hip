@@ -267,6 +267,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   }
 
   // ---- epilogue: O[i][d] = O^T[d][i] / l
+  const MgldMaskAttn& pe = D == 128 ? ma_late_args() : p;
   const float l = rs.l + __shfl_xor(rs.l, 32, 64);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float z = 0.f;
@@ -274,19 +275,20 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) z += rs.o[dt][r] * 0.f;
-  const unsigned long long bz = __ballot(z != z);      // an infinity or NaN came in
+  // an infinity or NaN came in, perhaps of a value that the row does not see.  (Where the sum of the probabilities is not finite, a score that it sees was not: all NaN.)
+  const unsigned long long bz = __ballot(z != z && l - l == 0.f);
   unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
-  if (i < p.Nq) {
-    if (p.lse && lhi == 0) p.lse[((int64_t)b * p.heads + h) * p.Nq + i] = l == 0.f ? -MA_INF : (rs.unit() + __builtin_amdgcn_logf(l)) * MA_LN2;
+  if (i < pe.Nq) {
+    if (pe.lse && lhi == 0) pe.lse[((int64_t)b * pe.heads + h) * pe.Nq + i] = l == 0.f ? -MA_INF : (rs.unit() + __builtin_amdgcn_logf(l)) * MA_LN2;
     if (!((bad >> l31) & 1)) {
-      T* const o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
+      T* const o = (T*)pe.O + b * pe.o_sb + (int64_t)i * pe.o_si + h * pe.o_sh;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int rg = 0; rg < 4; ++rg) {
           const int d = dt * 32 + rg * 8 + lhi * 4;
           typedef T t4 __attribute__((ext_vector_type(4)));
-          if (d < p.head_dim)
+          if (d < pe.head_dim)
             *(t4*)(o + d) = t4{(T)(rs.o[dt][rg * 4] * inv), (T)(rs.o[dt][rg * 4 + 1] * inv), (T)(rs.o[dt][rg * 4 + 2] * inv), (T)(rs.o[dt][rg * 4 + 3] * inv)};
         }
     }
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   while (bad) {
     const int r = __builtin_ctz(bad);
     bad &= bad - 1;
-    if (iw + r < p.Nq) ma_slow_row<T>(D == 128 ? ma_late_args() : p, b, h, iw + r);
+    if (iw + r < pe.Nq) ma_slow_row<T>(D == 128 ? ma_late_args() : p, b, h, iw + r);
   }
 }
 
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
       if (D == 128) po[lane + 64] = a1;
       if (lane == 0) { po[D] = M; po[D + 1] = L; }           // the maximum in log2 units
     } else {
-      const bool bad = __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f);
+      const bool bad = L - L == 0.f && __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f);      // (L not finite: a visible score was not, all NaN)
       if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + hh) * p.Nq + ii] = L == 0.f ? -MA_INF : (M + __builtin_amdgcn_logf(L)) * MA_LN2;
       if (bad) ma_slow_row<T>(p, b, hh, ii);
       else {
@@ -487,7 +489,7 @@ __global__ __launch_bounds__(64) void ma_join_kernel(const MgldMaskAttn p, const
   }
   const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.heads), b = (int)(row / p.Nq / p.heads);
   if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -MA_INF : (M + __builtin_amdgcn_logf(L)) * MA_LN2;
-  if (__any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f)) {
+  if (L - L == 0.f && __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f)) {
     ma_slow_row<T>(p, b, h, i);
     return;
   }

@@ -289,7 +289,8 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) z += o[dt][r] * 0.f;
-  const unsigned long long bz = __ballot(z != z);      // an infinity or NaN came in: perhaps by a key that the row does not see
+  // an infinity or NaN came in, perhaps by a key that the row does not see.  (Where D or lse is not finite, something that it sees was not: all NaN.)
+  const unsigned long long bz = __ballot(z != z && delta - delta == 0.f && lse == lse);
   unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
   if (rok && !((bad >> l31) & 1)) {
     const float f = p.scale / up;

@@ -294,6 +294,24 @@ def test_row_by_row_forms_under_any_cap(hip, name, dt, cap):
         check(n, torch.where(m, x.cpu().double(), res[n]), res[n], tol[n])
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), "row"])
+@pytest.mark.parametrize("name,dt,key", [("docs", F16, 100), ("text", F16, 40), ("d128", BF16, 70), ("cap", BF16, 64), ("tokens", BF16, 690), ("token_long", F16, 3000), ("d72", F16, 66)])
+def test_a_bad_value_that_rows_see(hip, name, dt, key, bad):
+    """an infinity or NaN in some columns of one value shows in those columns of the rows that see it, and nowhere else; a value row of NaN makes them NaN"""
+    q, k, v, do, kw = problem(name, dt, seed=20)
+    res, tol = reference(q, k, v, do, kw, grads=False)
+    vis, _ = tr.visible(q.shape[0], q.shape[1], k.shape[1], kw["causal"], kw.get("docs"), kw.get("prefix"), kw.get("kv_len"), kw.get("q_pos0"))
+    cols = slice(None) if bad == "row" else [1, q.shape[3] - 1]
+    v[:, key, :, cols] = float("nan") if bad == "row" else bad
+    o, lse = hip.masked_attention(q.to(DEV), k.to(DEV), v.to(DEV), **on_gpu(kw))
+    check_lse(lse, res["lse"], tol["lse"])
+    o, hit = o.cpu(), torch.zeros(res["o"].shape, dtype=torch.bool)
+    hit[:, :, :, cols] = vis[:, :, key, None, None]
+    assert bool(hit.any())
+    check("o", torch.where(hit, res["o"], o.double()), res["o"], tol["o"])
+    assert torch.isnan(o[hit]).all() if bad == "row" or bad != bad else (o[hit] == bad).all()
+
+
 # ---- many small probabilities ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [F16, BF16])
 @pytest.mark.parametrize("Nq,H", [(1, 1), (130, 40)])
