@@ -398,49 +398,49 @@ struct ExactRow {
       if (lane + 64 < d) a1 += wc * (float)r[lane + 64];
     }
   }
+  __device__ __forceinline__ T* at(void* out, const int64_t sb, const int64_t si, const int64_t sh) const { return (T*)out + b * sb + (int64_t)i * si + h * sh; }
   __device__ __forceinline__ void put(void* out, const int64_t sb, const int64_t si, const int64_t sh, const float a0, const float a1) const {
     const int lane = threadIdx.x & 63;
-    T* const o = (T*)out + b * sb + (int64_t)i * si + h * sh;
+    T* const o = at(out, sb, si, sh);
     if (lane < d) o[lane] = (T)a0;
     if (lane + 64 < d) o[lane + 64] = (T)a1;
   }
 };
-// Do the values that the row sees hold a NaN in every column?  Then so does the row, and nothing has to be computed: in a run that diverged every row is one of
-// these (4096 tokens, 32 / 8 heads of 128: 223 ms without this look, which reads V alone and mostly ends at its first rows).
+// Is the row's fast result, stored at `out`, not finite only where a row of `rows` (V for o, K for dQ) that it sees is not finite either, in the same column?  Then it stands:
+// in a run that diverged every row is one of these (4096 tokens, 32 / 8 heads of 128: 223 ms without this look, which mostly ends at its first rows).  A NaN of o needs a NaN,
+// an infinity an infinity (the weights are positive); dQ's weights may be zero or of either sign, so there one does for the other.
 template <typename T>
-__device__ __forceinline__ bool ma_sees_only_nan(const ExactRow<T>& row, const int64_t stride) {
-  constexpr unsigned EXP = __is_same(T, f16) ? 0x7c00u : 0x7f80u;      // magnitude bits above these: NaN
+__device__ __forceinline__ bool ma_stands(const ExactRow<T>& row, const T* rows, const int64_t stride, const T* out, const bool either) {
+  constexpr unsigned EXP = __is_same(T, f16) ? 0x7c00u : 0x7f80u;      // magnitude bits: of infinity; above: NaN
   const int lane = threadIdx.x & 63;
-  auto mag = [&](const int j, const int c) __attribute__((always_inline)) {
-    return lane + 64 * c < row.d ? ((const unsigned short*)row.vb)[(int64_t)j * stride + lane + 64 * c] & 0x7fffu : 0u;
-  };
-  bool n0 = lane >= row.d, n1 = lane + 64 >= row.d;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");              // (the wave's own stores are read back)
+  auto mag = [&](const T* x, const int c) __attribute__((always_inline)) { return lane + 64 * c < row.d ? ((const unsigned short*)x)[lane + 64 * c] & 0x7fffu : 0u; };
+  const unsigned o0 = mag(out, 0), o1 = mag(out, 1), t0 = o0 > EXP && !either ? EXP + 1 : EXP, t1 = o1 > EXP && !either ? EXP + 1 : EXP;
+  bool ok0 = o0 < EXP, ok1 = o1 < EXP;
   for (int j0 = 0; j0 < row.lim; j0 += 8) {
     unsigned top = 0;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const int j = min(j0 + u, row.lim - 1);
-      top = max(top, max(mag(j, 0), mag(j, 1)));
+      const T* const x = rows + (int64_t)min(j0 + u, row.lim - 1) * stride;
+      top = max(top, max(mag(x, 0), mag(x, 1)));
     }
-    if (!__any(top > EXP)) continue;
+    if (!__any(top >= EXP)) continue;
     const int j1 = min(j0 + 8, row.lim);
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
       if (!row.seen(j)) continue;
-      n0 = n0 || mag(j, 0) > EXP;
-      n1 = n1 || mag(j, 1) > EXP;
+      const T* const x = rows + (int64_t)j * stride;
+      ok0 = ok0 || mag(x, 0) >= t0;
+      ok1 = ok1 || mag(x, 1) >= t1;
     }
-    if (__all(n0 && n1)) return true;
+    if (__all(ok0 && ok1)) return true;
   }
   return false;
 }
 template <typename T>
 __device__ __forceinline__ void ma_slow_row(const MgldMaskAttn& p, const int b, const int h, const int i) {
   const ExactRow<T> row(p, b, h, i);
-  if (ma_sees_only_nan(row, p.v_si)) {
-    row.put(p.O, p.o_sb, p.o_si, p.o_sh, __builtin_nanf(""), __builtin_nanf(""));
-    return;
-  }
+  if (ma_stands(row, row.vb, p.v_si, (const T*)row.at(p.O, p.o_sb, p.o_si, p.o_sh), false)) return;
   const int lane = threadIdx.x & 63;
   float m = -MA_INF, sl;
   for (int j = lane; j < row.lim; j += 64)
@@ -463,6 +463,7 @@ template <typename T>
 __device__ __forceinline__ void ma_slow_dq(const MgldMaskAttn& p, const int b, const int h, const int i, const float lse2, const float delta) {
   const ExactRow<T> row(p, b, h, i);
   const int lane = threadIdx.x & 63;
+  if (ma_stands(row, row.kb, p.k_si, (const T*)row.at(p.dQ, p.dq_sb, p.dq_si, p.dq_sh), true)) return;
   const T* const g = (const T*)p.dO + b * p.do_sb + (int64_t)i * p.do_si + h * p.do_sh;
   float a0 = 0.f, a1 = 0.f;
   for (int j0 = 0; j0 < row.lim; j0 += 64) {

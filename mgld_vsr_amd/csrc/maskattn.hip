@@ -280,18 +280,16 @@ __global__ __launch_bounds__(256, D == 64 && !((MODE & MA_CAP) && MODE != MA_CAP
   unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
   if (i < pe.Nq) {
     if (pe.lse && lhi == 0) pe.lse[((int64_t)b * pe.heads + h) * pe.Nq + i] = l == 0.f ? -MA_INF : (rs.unit() + __builtin_amdgcn_logf(l)) * MA_LN2;
-    if (!((bad >> l31) & 1)) {
-      T* const o = (T*)pe.O + b * pe.o_sb + (int64_t)i * pe.o_si + h * pe.o_sh;
+    T* const o = (T*)pe.O + b * pe.o_sb + (int64_t)i * pe.o_si + h * pe.o_sh;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int rg = 0; rg < 4; ++rg) {
-          const int d = dt * 32 + rg * 8 + lhi * 4;
-          typedef T t4 __attribute__((ext_vector_type(4)));
-          if (d < pe.head_dim)
-            *(t4*)(o + d) = t4{(T)(rs.o[dt][rg * 4] * inv), (T)(rs.o[dt][rg * 4 + 1] * inv), (T)(rs.o[dt][rg * 4 + 2] * inv), (T)(rs.o[dt][rg * 4 + 3] * inv)};
-        }
-    }
+      for (int rg = 0; rg < 4; ++rg) {
+        const int d = dt * 32 + rg * 8 + lhi * 4;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        if (d < pe.head_dim)
+          *(t4*)(o + d) = t4{(T)(rs.o[dt][rg * 4] * inv), (T)(rs.o[dt][rg * 4 + 1] * inv), (T)(rs.o[dt][rg * 4 + 2] * inv), (T)(rs.o[dt][rg * 4 + 3] * inv)};
+      }
   }
   while (bad) {
     const int r = __builtin_ctz(bad);
@@ -459,13 +457,11 @@ __global__ __launch_bounds__(256, 2) void ma_split_kernel(const MgldMaskAttn p, 
     } else {
       const bool bad = L - L == 0.f && __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f);      // (L not finite: a visible score was not, all NaN)
       if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + hh) * p.Nq + ii] = L == 0.f ? -MA_INF : (M + __builtin_amdgcn_logf(L)) * MA_LN2;
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      T* const o = (T*)p.O + b * p.o_sb + (int64_t)ii * p.o_si + hh * p.o_sh;
+      if (lane < p.head_dim) o[lane] = (T)(a0 * inv);
+      if (lane + 64 < p.head_dim) o[lane + 64] = (T)(a1 * inv);
       if (bad) ma_slow_row<T>(p, b, hh, ii);
-      else {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        T* const o = (T*)p.O + b * p.o_sb + (int64_t)ii * p.o_si + hh * p.o_sh;
-        if (lane < p.head_dim) o[lane] = (T)(a0 * inv);
-        if (lane + 64 < p.head_dim) o[lane + 64] = (T)(a1 * inv);
-      }
     }
   }
 }
@@ -489,14 +485,11 @@ __global__ __launch_bounds__(64) void ma_join_kernel(const MgldMaskAttn p, const
   }
   const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.heads), b = (int)(row / p.Nq / p.heads);
   if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -MA_INF : (M + __builtin_amdgcn_logf(L)) * MA_LN2;
-  if (L - L == 0.f && __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f)) {
-    ma_slow_row<T>(p, b, h, i);
-    return;
-  }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   T* const o = (T*)p.O + b * p.o_sb + (int64_t)i * p.o_si + h * p.o_sh;
   if (lane < p.head_dim) o[lane] = (T)(a0 * inv);
   if (lane + 64 < p.head_dim) o[lane + 64] = (T)(a1 * inv);
+  if (L - L == 0.f && __any(a0 * 0.f != a0 * 0.f || a1 * 0.f != a1 * 0.f)) ma_slow_row<T>(p, b, h, i);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------

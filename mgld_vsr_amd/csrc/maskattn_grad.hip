@@ -292,7 +292,7 @@ __global__ __launch_bounds__(256, 2) void ma_dq_kernel(const MgldMaskAttn p, con
   // an infinity or NaN came in, perhaps by a key that the row does not see.  (Where D or lse is not finite, something that it sees was not: all NaN.)
   const unsigned long long bz = __ballot(z != z && delta - delta == 0.f && lse == lse);
   unsigned bad = (unsigned)bz | (unsigned)(bz >> 32);
-  if (rok && !((bad >> l31) & 1)) {
+  if (rok) {
     const float f = p.scale / up;
     T* const out = (T*)p.dQ + b * p.dq_sb + (int64_t)i * p.dq_si + h * p.dq_sh;
 #pragma unroll

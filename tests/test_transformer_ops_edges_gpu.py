@@ -262,9 +262,9 @@ def test_dq_depends_on_what_its_row_sees_alone(hip, name, dt, key):
     q, k, v, do, kw = problem(name, dt, seed=18)
     res, tol = reference(q, k, v, do, kw)
     vis, _ = tr.visible(q.shape[0], q.shape[1], k.shape[1], kw["causal"], kw.get("docs"), kw.get("prefix"), kw.get("kv_len"), kw.get("q_pos0"))
-    for x, bad in ((k, float("nan")), (v, float("inf"))):
+    for x, bad, cols in ((k, float("nan"), slice(None)), (v, float("inf"), slice(None)), (k, float("inf"), [2]), (k, float("nan"), [0, 5]), (v, float("nan"), [1])):
         kb, vb = k.clone(), v.clone()
-        (kb if x is k else vb)[:, key] = bad
+        (kb if x is k else vb)[:, key, :, cols] = bad
         _, _, grads = run(hip, q, kb, vb, do, kw)
         blind = ~vis[:, :, key]
         m = blind[:, :, None, None].expand_as(res["dq"])
