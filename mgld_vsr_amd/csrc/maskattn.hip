@@ -14,7 +14,7 @@
 //
 // Bounds and figures (4 d products per visible pair; a large matrix product reaches 1400 TFLOP/s):
 //  * many rows, d = 128: 880-905 TFLOP/s on full tiles, 750-780 under a cap (three transcendentals per score), ~740 at d = 64; ~10 us a launch beside that.
-//    8192 tokens, 32 / 8 heads of 128, causal, cap 50: 707 us.  Neither pipe is full there: the vector pipe is active 72 % of the cycles, the matrix pipe 35 %, and waves
+//    8192 tokens, 32 / 8 heads of 128, causal, cap 50: 697 us.  Neither pipe is full there: the vector pipe is active 72 % of the cycles, the matrix pipe 35 %, and waves
 //    wait 21 % of theirs: the chain from a score over its exponentials to the second product, with two waves per SIMD to hide it.  128 rows a block =
 //    two blocks per CU (three at d = 64), so one's barrier is the other's work.
 //    Keeping unscaled scores (32 of 340 vector instructions fewer per tile) gained 0.8 % and spilled at d = 64; one m0 write for several DMA pieces: nothing.
